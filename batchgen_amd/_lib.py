@@ -110,6 +110,22 @@ _SIGS = {
                                               i64, vp, sz, vp]),
     "bgmoe_fp8_fused_s1_balanced": (i32, [C.POINTER(Fp8Act), C.POINTER(Fp8Weight), C.POINTER(Fp8Weight), vp, vp, i32,
                                           i64, i32, i32, vp, vp, vp, i64, i64, i64, vp, sz, vp]),
+    "bgmoe_int8_quant_rows": (i32, [vp, i32, i64, i64, i32, vp, vp, vp]),
+    "bgmoe_int8_gemm_workspace_bytes": (sz, [i64, i32, i32]),
+    "bgmoe_int8_gemm": (i32, [vp, i64, vp, vp, vp, vp, i64, i32, i32, vp, i32, i64, vp, sz, vp]),
+    "bgmoe_int8_linear_workspace_bytes": (sz, [i64, i32, i32]),
+    "bgmoe_int8_linear": (i32, [vp, i32, i64, vp, vp, vp, i64, i32, i32, vp, i32, i64, vp, sz, vp]),
+    "bgmoe_int8_grouped_gemm": (i32, [vp, vp, vp, i64, vp, i64, vp, vp, i32, i64, i32, i32, vp, i32, vp]),
+    "bgmoe_int8_fused_s1": (i32, [vp, vp, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, i32, i64, i32, i32, vp, i32, vp]),
+    "bgmoe_token_sort_index": (i32, [vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, sz, vp]),
+    "bgmoe_token_sort_rows": (i32, [vp, i64, i64, i32, i32, vp, vp, vp, i32, i64, i32, vp, vp]),
+    "bgmoe_token_unsort": (i32, [vp, i32, vp, vp, i32, i32, i32, vp, vp]),
+    "bgmoe_token_unsort_backward": (i32, [vp, vp, i32, vp, vp, i32, i32, i32, vp, vp, i32, i64, vp, vp, vp]),
+    "bgmoe_gated_residual_norm": (i32, [vp, vp, i32, vp, vp, i32, f32, vp, i32, i64, i32, f32, vp, vp, vp, vp, vp, vp,
+                                        vp]),
+    "bgmoe_gated_residual_norm_backward_workspace_bytes": (sz, [i64, i32]),
+    "bgmoe_gated_residual_norm_backward": (i32, [vp, vp, i32, vp, vp, i32, f32, vp, i32, i64, i32, vp, vp, vp, vp, vp, vp,
+                                                 vp, vp, vp, vp, sz, vp]),
 }
 
 _lib = None

@@ -10,6 +10,7 @@
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef int intx8 __attribute__((ext_vector_type(8)));
 typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef int intx16 __attribute__((ext_vector_type(16)));
 typedef short shortx8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
@@ -50,6 +51,7 @@ enum BgmoeKernelId {
   BGMOE_K_GEMM_SKINNY16, BGMOE_K_GEMM_SKINNY64, BGMOE_K_GEMM_TILED,
   BGMOE_K_MXFP4_S1, BGMOE_K_MXFP4_GEMM, BGMOE_K_BF16_GEMM, BGMOE_K_ROUTER_GEMM, BGMOE_K_ROUTER_GEMM_REDUCE,
   BGMOE_K_NORM_QUANT, BGMOE_K_SITU, BGMOE_K_DENSE_GEMM,
+  BGMOE_K_TOKEN_SORT, BGMOE_K_TOKEN_UNSORT, BGMOE_K_GATED_NORM, BGMOE_K_INT8_QUANT, BGMOE_K_INT8_GEMM,
   BGMOE_K_COUNT
 };
 extern bool g_bgmoe_prof_on;
@@ -66,6 +68,7 @@ int bgmoe_internal_init_fp8_tiled();
 int bgmoe_internal_init_mxfp4();
 int bgmoe_internal_init_router_gemm();
 int bgmoe_internal_init_permute();
+int bgmoe_internal_init_int8_gemm();
 int bgmoe_internal_fp8_gemm(const bgmoe_fp8_act* a, const bgmoe_fp8_weight* w0, const bgmoe_fp8_weight* w1,
                             const int32_t* seqlens, const int32_t* cu, int groups, int64_t m, int n, int k,
                             uint16_t* out, uint8_t* out_q, float* out_s, int64_t os_row, int64_t os_nb,

@@ -1,0 +1,468 @@
+// Products in 8-bit integers for gfx950: out[t][j] = (sum_k x[t][k] w[j][k]) * xs[t] * ws[j], dense or grouped by
+// expert, and the row quantiser in front of them.
+//
+// Both operands are K-major rows, which is what v_mfma_i32_16x16x64_i8 takes: lane l = 16 q + r supplies the 16 bytes
+// k = 16 q .. 16 q + 15 of row r.  With the weights as first operand a lane's four results are four consecutive output
+// columns of one token.  The accumulators are exact 32-bit integers (|sum| <= k * 128^2 < 2^31 for k <= 131071), so
+// no result depends on how K is cut; the scales enter once, in fp32, in the epilogue.
+//
+// Streaming kernel: a block owns 64 weight rows (4 waves x 16) and all of K, and walks the group's tokens in chunks of
+// 16, 32 or 64.  Weights and tokens go global -> LDS asynchronously in stages of 256 bytes of K (one 1 KB wave load
+// covers 4 rows x 256 contiguous bytes) into a ring; a stage's 16-byte chunks are stored at position
+// chunk ^ (row & 15), so that the 16 lanes that read one chunk of 16 rows hit 16 different 16-byte slots of the 256
+// bytes the LDS serves at once.
+#include "bgmoe_async.h"
+#include "bgmoe_elem.h"
+
+namespace {
+
+constexpr int kMaxK = 131071;                 // k * 128 * 128 < 2^31
+constexpr int kStageK = 256;                  // bytes of K per stage
+constexpr int kTile = 16 * kStageK;           // 16 rows of a stage: 4 KB
+constexpr int kRingBytes = 80 * 1024;         // two blocks per CU
+
+__device__ const uint4 g_zeros = {0u, 0u, 0u, 0u};     // what chunks past K read
+
+struct Int8Args {
+  const int8_t* x;
+  int64_t ldx;                                // bytes between rows of x
+  const float* xs;
+  const int8_t *w0, *w1;                      // w1: the up projection of a fused stage 1, else null
+  int64_t w0_group, w1_group;
+  const float *ws0, *ws1;
+  int64_t ws0_group, ws1_group;
+  const float* bias;
+  const int32_t *seqlens, *cu;                // null: one group of all m rows
+  int64_t m;
+  int n, k;
+  uint8_t* out;
+  int64_t ldo;                                // elements between rows of out
+  int out_dtype;
+};
+
+// four consecutive columns of one output row
+__device__ __forceinline__ void store4(const Int8Args& a, int64_t row, int col, const float (&v)[4]) {
+  const int left = a.n - col;
+  if (left <= 0) return;
+  typedef unsigned int u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+  if (a.out_dtype == BGMOE_DT_FP32) {
+    float* p = reinterpret_cast<float*>(a.out) + row * a.ldo + col;
+    if (left >= 4) store16(p, u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
+    else for (int i = 0; i < left; ++i) p[i] = v[i];
+    return;
+  }
+  uint16_t* p = reinterpret_cast<uint16_t*>(a.out) + row * a.ldo + col;
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    b[i] = a.out_dtype == BGMOE_DT_BF16 ? f32_to_bf16_bits(v[i]) : (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[i]);
+  if (left >= 4) *reinterpret_cast<u32x2_any*>(p) = u32x2_any{b[0] | (b[1] << 16), b[2] | (b[3] << 16)};
+  else for (int i = 0; i < left; ++i) p[i] = (uint16_t)b[i];
+}
+
+// rows [row0, row0 + cnt) of group g; counts and offsets that reach outside [0, m] are cut
+__device__ __forceinline__ void group_rows(const Int8Args& a, int g, int64_t* row0, int* cnt) {
+  if (a.seqlens == nullptr) {
+    *row0 = 0;
+    *cnt = (int)a.m;
+    return;
+  }
+  const int64_t r = a.cu[g];
+  const int64_t end = min(r + (int64_t)a.seqlens[g], a.m);
+  *row0 = r;
+  *cnt = r >= 0 && end > r ? (int)(end - r) : 0;
+}
+
+template <bool FUSED, int MT>
+__device__ __forceinline__ void stream_chunk(const Int8Args& a, uint8_t* smem, const int8_t* wbase, int wrow0, int wrows,
+                                             const float* ws, const float* ws_up, int64_t row0, int t0, int cnt, int n0) {
+  constexpr int kStage = (4 + MT) * kTile;             // 64 weight rows, 16 MT tokens
+  constexpr int kStages = kRingBytes / kStage;         // 4, 3, 2
+  constexpr int kLoads = 4 + MT;                       // wave loads per stage and wave
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int r = lane & 15, q = lane >> 4;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
+  const int S = (a.k + kStageK - 1) / kStageK;
+  const int chunks = a.k >> 4;                          // 16-byte chunks of a row
+
+  // sources: lane l of wave load i covers row 4 i + l/16 of the tile, LDS position l % 16, i.e. source chunk
+  // (l % 16) ^ (row & 15)
+  const int lr = lane >> 4, lc = lane & 15;
+  uint32_t w_off[4], x_off[MT];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 4 * i + lr;
+    w_off[i] = (uint32_t)min(row, wrows - 1) * (uint32_t)a.k + (uint32_t)((lc ^ row) * 16);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int row = 4 * (wave * MT + i) + lr;           // token of the chunk
+    x_off[i] = (uint32_t)min(row, cnt - 1 - t0) * (uint32_t)a.ldx + (uint32_t)((lc ^ (row & 15)) * 16);
+  }
+  const uint8_t* wsrc = uniform_ptr(reinterpret_cast<const uint8_t*>(wbase) + (int64_t)wrow0 * a.k);
+  const uint8_t* xsrc = uniform_ptr(reinterpret_cast<const uint8_t*>(a.x) + (row0 + t0) * a.ldx);
+
+  auto issue = [&](int s) {
+    const uint32_t d = lds0 + (uint32_t)(s % kStages) * kStage;
+    const uint32_t dw = d + wave * kTile, dx = d + 4 * kTile + wave * MT * 1024;
+    const int ko = s * kStageK;
+    if ((s + 1) * 16 <= chunks) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) async_load16(wsrc + ko, w_off[i], dw + i * 1024);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) async_load16(xsrc + ko, x_off[i], dx + i * 1024);
+    } else {                                            // the last, partial stage: chunks past K read zeros
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool in = s * 16 + (lc ^ (4 * i + lr)) < chunks;
+        async_load16_lane(in ? (const void*)(wsrc + ko + w_off[i]) : (const void*)&g_zeros, dw + i * 1024);
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const bool in = s * 16 + (lc ^ ((4 * (wave * MT + i) + lr) & 15)) < chunks;
+        async_load16_lane(in ? (const void*)(xsrc + ko + x_off[i]) : (const void*)&g_zeros, dx + i * 1024);
+      }
+    }
+  };
+
+  intx4 acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) acc[t] = intx4{0, 0, 0, 0};
+  for (int s = 0; s < kStages - 1 && s < S; ++s) issue(s);
+  for (int s = 0; s < S; ++s) {
+    // stages s + 1 .. s + kStages - 2 may still be in flight
+    if (S - 1 - s >= kStages - 2) wait_vm<(kStages - 2) * kLoads>();
+    else wait_vm<0>();
+    lds_exchange_barrier();                             // everybody's share has landed; everybody is done with stage s - 1
+    if (s + kStages - 1 < S) issue(s + kStages - 1);
+    const uint8_t* b = smem + (s % kStages) * kStage;
+    const uint8_t* bw = b + wave * kTile + r * kStageK;
+    const uint8_t* bx = b + 4 * kTile + r * kStageK;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int o = ((4 * c + q) ^ r) * 16;
+      const intx4 wv = *reinterpret_cast<const intx4*>(bw + o);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+        acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv, *reinterpret_cast<const intx4*>(bx + t * kTile + o), acc[t], 0, 0, 0);
+    }
+  }
+  lds_exchange_barrier();                               // the ring is free
+
+  // epilogue: lane (r, q) holds columns 4 q .. 4 q + 3 of this wave's 16 for token r of each 16-token tile
+  if constexpr (FUSED) {
+    // waves 0, 1: gate rows, waves 2, 3: the up rows of the same columns, handed over through LDS
+    float* up = reinterpret_cast<float*>(smem);
+    const int col = n0 + (wave & 1) * 16 + 4 * q;
+    float sc[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sc[i] = (wave < 2 ? ws : ws_up)[min(col + i, a.n - 1)];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const float xs = a.xs[row0 + min(t0 + 16 * t + r, cnt - 1)];
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (float)acc[t][i] * xs * sc[i];
+      if (wave >= 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) up[(((wave & 1) * MT + t) * 4 + i) * 64 + lane] = v[i];
+      else
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] = __float_as_int(v[i]);
+    }
+    __syncthreads();
+    if (wave < 2) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[i] = silu_f32(__int_as_float(acc[t][i])) * up[((wave * MT + t) * 4 + i) * 64 + lane];
+        const int tok = t0 + 16 * t + r;
+        if (tok < cnt) store4(a, row0 + tok, col, v);
+      }
+    }
+    __syncthreads();
+  } else {
+    const int col = n0 + wave * 16 + 4 * q;
+    float sc[4], bias[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sc[i] = ws[min(col + i, a.n - 1)];
+      bias[i] = a.bias ? a.bias[min(col + i, a.n - 1)] : 0.0f;
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const int tok = t0 + 16 * t + r;
+      if (tok >= cnt) continue;
+      const float xs = a.xs[row0 + tok];
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = (float)acc[t][i] * xs * sc[i];
+        if (a.bias) v[i] += bias[i];
+      }
+      store4(a, row0 + tok, col, v);
+    }
+  }
+}
+
+template <bool FUSED>
+__global__ __launch_bounds__(256) void int8_stream_kernel(Int8Args a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int g = blockIdx.y;
+  int64_t row0;
+  int cnt;
+  group_rows(a, g, &row0, &cnt);
+  if (cnt == 0) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * (FUSED ? 32 : 64);
+  const bool second = FUSED && wave >= 2;
+  const int8_t* wbase = second ? a.w1 + g * a.w1_group : a.w0 + g * a.w0_group;
+  const float* ws = a.ws0 + g * a.ws0_group;
+  const float* ws_up = FUSED ? a.ws1 + g * a.ws1_group : nullptr;
+  // this wave's 16 weight rows; a wave whose rows all lie past n repeats the last row and stores nothing
+  const int wrow0 = min(n0 + (FUSED ? wave & 1 : wave) * 16, a.n - 1);
+  const int wrows = min(16, a.n - wrow0);
+  for (int t0 = 0; t0 < cnt;) {
+    const int left = cnt - t0;
+    if (left <= 16) {
+      stream_chunk<FUSED, 1>(a, smem, wbase, wrow0, wrows, ws, ws_up, row0, t0, cnt, n0);
+      t0 += 16;
+    } else if (left <= 32) {
+      stream_chunk<FUSED, 2>(a, smem, wbase, wrow0, wrows, ws, ws_up, row0, t0, cnt, n0);
+      t0 += 32;
+    } else {
+      stream_chunk<FUSED, 4>(a, smem, wbase, wrow0, wrows, ws, ws_up, row0, t0, cnt, n0);
+      t0 += 64;
+    }
+  }
+}
+
+// ---- row quantiser: one block per row, the row in registers between its maximum and its cast -----------------------------
+template <typename T, int V>
+__global__ __launch_bounds__(1024) void int8_quant_kernel(const uint8_t* __restrict__ x, int64_t stride, int64_t rows,
+                                                          int k, int8_t* __restrict__ q, float* __restrict__ scale) {
+  __shared__ float s_max[16];
+  const int64_t row = linear_block();
+  if (row >= rows) return;
+  const uint8_t* src = x + row * stride * T::kBytes;
+  const int step = blockDim.x * 8;
+  float v[V > 0 ? V : 1][8];
+  float amax = 0.0f;
+  bool bad = false;
+  auto take = [&](const float (&w)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      amax = fmaxf(amax, fabsf(w[i]));
+      bad = bad || w[i] != w[i];                        // fmaxf drops a NaN
+    }
+  };
+  if constexpr (V > 0) {
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      const int c = threadIdx.x * 8 + u * step;
+      load8<T>(src, c, k - c, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < V; ++u) take(v[u]);
+  } else {                                              // a row longer than the registers hold is read twice
+    for (int c = threadIdx.x * 8; c < k; c += step) {
+      load8<T>(src, c, k - c, v[0]);
+      take(v[0]);
+    }
+  }
+  if (bad) amax = __builtin_huge_valf();
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, BGMOE_WAVE));
+  const int waves = blockDim.x >> 6;
+  if (waves > 1) {
+    if (lane_id() == 0) s_max[threadIdx.x >> 6] = amax;
+    __syncthreads();
+    amax = s_max[0];
+    for (int w = 1; w < waves; ++w) amax = fmaxf(amax, s_max[w]);
+  }
+  const float sc = int8_scale(amax);
+  if (threadIdx.x == 0) scale[row] = sc;
+  int8_t* dst = q + row * k;
+  if constexpr (V > 0) {
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      const int c = threadIdx.x * 8 + u * step;
+      int8_store8(dst + c, k - c, v[u], sc);
+    }
+  } else {
+    for (int c = threadIdx.x * 8; c < k; c += step) {
+      load8<T>(src, c, k - c, v[0]);
+      int8_store8(dst + c, k - c, v[0], sc);
+    }
+  }
+}
+
+template <typename T>
+int run_quant(const void* x, int64_t stride, int64_t rows, int k, int8_t* q, float* scale, hipStream_t st) {
+  const int vecs = k <= 8192 ? 1 : (k <= 16384 ? 2 : 0);
+  int threads = 1024;
+  if (vecs) threads = ((k + 8 * vecs - 1) / (8 * vecs) + BGMOE_WAVE - 1) / BGMOE_WAVE * BGMOE_WAVE;
+  const dim3 grid = bgmoe_grid(rows), block(threads);
+  BgmoeProf prof(BGMOE_K_INT8_QUANT, st);
+  if (vecs == 1) hipLaunchKernelGGL((int8_quant_kernel<T, 1>), grid, block, 0, st, (const uint8_t*)x, stride, rows, k, q, scale);
+  else if (vecs == 2) hipLaunchKernelGGL((int8_quant_kernel<T, 2>), grid, block, 0, st, (const uint8_t*)x, stride, rows, k, q, scale);
+  else hipLaunchKernelGGL((int8_quant_kernel<T, 0>), grid, block, 0, st, (const uint8_t*)x, stride, rows, k, q, scale);
+  return bgmoe_check_launch("int8_quant_rows");
+}
+
+int check_sizes(const char* what, int64_t m, int n, int k, int out_dtype) {
+  BGMOE_REQUIRE(m >= 0 && m <= 0x7fffffffLL && n >= 0, "%s: bad sizes m=%lld n=%d", what, (long long)m, n);
+  BGMOE_REQUIRE(k >= 16 && k <= kMaxK && k % 16 == 0, "%s: k=%d must be a multiple of 16 in [16, %d]", what, k, kMaxK);
+  BGMOE_REQUIRE(out_dtype >= BGMOE_DT_BF16 && out_dtype <= BGMOE_DT_FP32, "%s: unknown output type %d", what, out_dtype);
+  return BGMOE_OK;
+}
+
+int run_gemm(const char* what, const Int8Args& a, int groups, hipStream_t st) {
+  const bool fused = a.w1 != nullptr;
+  const int cols = fused ? 32 : 64;
+  const int64_t tiles = ((int64_t)a.n + cols - 1) / cols;
+  BGMOE_REQUIRE(tiles <= 1 << 24, "%s: n=%d is too wide", what, a.n);
+  const dim3 grid((unsigned)tiles, (unsigned)groups), block(256);
+  BgmoeProf prof(BGMOE_K_INT8_GEMM, st);
+  if (fused) hipLaunchKernelGGL(int8_stream_kernel<true>, grid, block, kRingBytes, st, a);
+  else hipLaunchKernelGGL(int8_stream_kernel<false>, grid, block, kRingBytes, st, a);
+  return bgmoe_check_launch(what);
+}
+
+}  // namespace
+
+int bgmoe_internal_init_int8_gemm() {
+  const void* fns[2] = {(const void*)int8_stream_kernel<false>, (const void*)int8_stream_kernel<true>};
+  for (const void* f : fns) {
+    const hipError_t err = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+    if (err != hipSuccess) {
+      bgmoe_set_error("int8 product: hipFuncSetAttribute(dynamic LDS) failed: %s", hipGetErrorString(err));
+      return BGMOE_ERR_HIP;
+    }
+  }
+  return BGMOE_OK;
+}
+
+// the dynamic-LDS opt-in holds per device: done once for each before its first launch
+static int ensure_init() {
+  static bool done[64] = {};
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) {
+    bgmoe_set_error("int8 product: no current HIP device (or device index >= 64)");
+    return BGMOE_ERR_HIP;
+  }
+  if (!done[dev]) {
+    const int rc = bgmoe_internal_init_int8_gemm();
+    if (rc != BGMOE_OK) return rc;
+    done[dev] = true;
+  }
+  return BGMOE_OK;
+}
+
+extern "C" int bgmoe_int8_quant_rows(const void* x, int dtype, int64_t x_row_stride, int64_t rows, int k, int8_t* q,
+                                     float* scale, bgmoe_stream_t stream) {
+  BGMOE_REQUIRE(dtype >= BGMOE_DT_BF16 && dtype <= BGMOE_DT_FP32, "int8_quant_rows: unknown element type %d", dtype);
+  BGMOE_REQUIRE(rows >= 0 && rows <= 0x7fffffffLL && k >= 0, "int8_quant_rows: bad sizes rows=%lld k=%d", (long long)rows, k);
+  if (rows == 0) return BGMOE_OK;
+  BGMOE_REQUIRE(k >= 1 && x && q && scale, "int8_quant_rows: null pointer or empty rows");
+#define BGMOE_CALL(T) run_quant<T>(x, x_row_stride, rows, k, q, scale, bgmoe_stream(stream))
+  BGMOE_BY_TYPE(dtype, BGMOE_CALL);
+#undef BGMOE_CALL
+}
+
+extern "C" size_t bgmoe_int8_gemm_workspace_bytes(int64_t m, int n, int k) {
+  (void)m; (void)n; (void)k;
+  return 0;
+}
+
+extern "C" int bgmoe_int8_gemm(const int8_t* x, int64_t x_row_stride, const float* x_scale, const int8_t* w,
+                               const float* w_scale, const float* bias, int64_t m, int n, int k, void* out, int out_dtype,
+                               int64_t out_row_stride, void* workspace, size_t workspace_bytes, bgmoe_stream_t stream) {
+  int rc = check_sizes("int8_gemm", m, n, k, out_dtype);
+  if (rc != BGMOE_OK) return rc;
+  if (m == 0 || n == 0) return BGMOE_OK;
+  BGMOE_REQUIRE(x && x_scale && w && w_scale && out, "int8_gemm: null pointer");
+  BGMOE_REQUIRE(((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_row_stride) % 16 == 0,
+                "int8_gemm: x, w and x_row_stride must be multiples of 16 bytes");
+  BGMOE_REQUIRE(x_row_stride >= k && x_row_stride < (1LL << 25), "int8_gemm: x_row_stride %lld outside [k, 2^25)",
+                (long long)x_row_stride);
+  BGMOE_REQUIRE(out_row_stride >= n, "int8_gemm: out_row_stride %lld is smaller than n=%d", (long long)out_row_stride, n);
+  (void)workspace; (void)workspace_bytes;
+  rc = ensure_init();
+  if (rc != BGMOE_OK) return rc;
+  Int8Args a{};
+  a.x = x; a.ldx = x_row_stride; a.xs = x_scale; a.w0 = w; a.ws0 = w_scale; a.bias = bias; a.m = m; a.n = n; a.k = k;
+  a.out = (uint8_t*)out; a.ldo = out_row_stride; a.out_dtype = out_dtype;
+  return run_gemm("int8_gemm", a, 1, bgmoe_stream(stream));
+}
+
+static size_t linear_rows_bytes(int64_t m, int k) { return ((size_t)m * (size_t)k + 15) / 16 * 16; }
+static size_t linear_scale_bytes(int64_t m) { return ((size_t)m * 4 + 15) / 16 * 16; }
+
+extern "C" size_t bgmoe_int8_linear_workspace_bytes(int64_t m, int n, int k) {
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  return linear_rows_bytes(m, k) + linear_scale_bytes(m) + bgmoe_int8_gemm_workspace_bytes(m, n, k);
+}
+
+extern "C" int bgmoe_int8_linear(const void* x, int x_dtype, int64_t x_row_stride, const int8_t* w, const float* w_scale,
+                                 const float* bias, int64_t m, int n, int k, void* out, int out_dtype,
+                                 int64_t out_row_stride, void* workspace, size_t workspace_bytes, bgmoe_stream_t stream) {
+  int rc = check_sizes("int8_linear", m, n, k, out_dtype);
+  if (rc != BGMOE_OK) return rc;
+  if (m == 0 || n == 0) return BGMOE_OK;
+  BGMOE_REQUIRE(x && w && w_scale && out, "int8_linear: null pointer");
+  const size_t need = bgmoe_int8_linear_workspace_bytes(m, n, k);
+  if (workspace == nullptr || workspace_bytes < need) {
+    bgmoe_set_error("int8_linear: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    return BGMOE_ERR_WORKSPACE;
+  }
+  BGMOE_REQUIRE((uintptr_t)workspace % 16 == 0, "int8_linear: workspace must be 16-byte aligned");
+  uint8_t* ws = (uint8_t*)workspace;
+  int8_t* q = (int8_t*)ws;
+  float* qs = (float*)(ws + linear_rows_bytes(m, k));
+  uint8_t* rest = ws + linear_rows_bytes(m, k) + linear_scale_bytes(m);
+  rc = bgmoe_int8_quant_rows(x, x_dtype, x_row_stride, m, k, q, qs, stream);
+  if (rc != BGMOE_OK) return rc;
+  return bgmoe_int8_gemm(q, k, qs, w, w_scale, bias, m, n, k, out, out_dtype, out_row_stride, rest,
+                         workspace_bytes - (size_t)(rest - ws), stream);
+}
+
+static int grouped(const char* what, Int8Args& a, int groups, int out_dtype, bgmoe_stream_t stream) {
+  int rc = check_sizes(what, a.m, a.n, a.k, out_dtype);
+  if (rc != BGMOE_OK) return rc;
+  BGMOE_REQUIRE(groups >= 1 && groups <= 65535, "%s: %d groups outside [1, 65535]", what, groups);
+  if (a.m == 0 || a.n == 0) return BGMOE_OK;
+  BGMOE_REQUIRE(a.x && a.xs && a.w0 && a.ws0 && a.seqlens && a.cu && a.out, "%s: null pointer", what);
+  BGMOE_REQUIRE(((uintptr_t)a.x | (uintptr_t)a.w0 | (uintptr_t)a.w0_group | (uintptr_t)a.w1 | (uintptr_t)a.w1_group) % 16 == 0,
+                "%s: x, weights and their group strides must be multiples of 16 bytes", what);
+  a.ldx = a.k; a.ldo = a.n; a.out_dtype = out_dtype;
+  rc = ensure_init();
+  if (rc != BGMOE_OK) return rc;
+  return run_gemm(what, a, groups, bgmoe_stream(stream));
+}
+
+extern "C" int bgmoe_int8_grouped_gemm(const int8_t* x, const float* x_scale, const int8_t* w, int64_t w_group_stride,
+                                       const float* w_scale, int64_t w_scale_group_stride, const int32_t* seqlens,
+                                       const int32_t* cu_seqlens, int groups, int64_t m, int n, int k, void* out,
+                                       int out_dtype, bgmoe_stream_t stream) {
+  Int8Args a{};
+  a.x = x; a.xs = x_scale; a.w0 = w; a.w0_group = w_group_stride; a.ws0 = w_scale; a.ws0_group = w_scale_group_stride;
+  a.seqlens = seqlens; a.cu = cu_seqlens; a.m = m; a.n = n; a.k = k; a.out = (uint8_t*)out;
+  return grouped("int8_grouped_gemm", a, groups, out_dtype, stream);
+}
+
+extern "C" int bgmoe_int8_fused_s1(const int8_t* x, const float* x_scale, const int8_t* gate, int64_t gate_group_stride,
+                                   const float* gate_scale, int64_t gate_scale_group_stride, const int8_t* up,
+                                   int64_t up_group_stride, const float* up_scale, int64_t up_scale_group_stride,
+                                   const int32_t* seqlens, const int32_t* cu_seqlens, int groups, int64_t m, int n, int k,
+                                   void* out, int out_dtype, bgmoe_stream_t stream) {
+  BGMOE_REQUIRE(m == 0 || n == 0 || (up && up_scale), "int8_fused_s1: null pointer");
+  Int8Args a{};
+  a.x = x; a.xs = x_scale; a.w0 = gate; a.w0_group = gate_group_stride; a.ws0 = gate_scale; a.ws0_group = gate_scale_group_stride;
+  a.w1 = up; a.w1_group = up_group_stride; a.ws1 = up_scale; a.ws1_group = up_scale_group_stride;
+  a.seqlens = seqlens; a.cu = cu_seqlens; a.m = m; a.n = n; a.k = k; a.out = (uint8_t*)out;
+  return grouped("int8_fused_s1", a, groups, out_dtype, stream);
+}

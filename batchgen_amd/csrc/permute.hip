@@ -21,6 +21,7 @@ constexpr int kMaxLocal = 1024;    // local experts
 
 struct PermArgs {
   const int32_t* ids;      // [nk]
+  const int64_t* ids64;    // [nk], used instead of ids when not null
   int64_t nk;
   int expert_start, e_local;
   int mtp;                 // masked layout stride, or 0 for ragged
@@ -51,7 +52,8 @@ __device__ __forceinline__ void write_tail(const PermArgs& a, int64_t off) {
 
 __device__ __forceinline__ int local_id(const PermArgs& a, int64_t i) {
   if (i >= a.nk) return -1;
-  const int64_t le = (int64_t)a.ids[i] - a.expert_start;
+  const int64_t id = a.ids64 != nullptr ? a.ids64[i] : (int64_t)a.ids[i];
+  const int64_t le = id - a.expert_start;
   return (le >= 0 && le < a.e_local) ? (int)le : -1;
 }
 
@@ -539,6 +541,28 @@ extern "C" int bgmoe_dispatch_index_3d(const int32_t* topk_ids, int n, int k, in
   a.e_local = num_local_experts; a.mtp = max_tokens_padded; a.row_align = 1;
   a.counts = expert_counts; a.counters = expert_counters; a.cu = nullptr; a.pos = topk_pos; a.row_pair = row_pair;
   a.extra_count = -1;
+  return run_index(a, workspace, workspace_bytes, bgmoe_stream(stream));
+}
+
+extern "C" int bgmoe_token_sort_index(const void* topk_ids, int ids_are_int64, int n, int k, int expert_start,
+                                      int num_local_experts, int row_align, int32_t* counts, int32_t* cu_seqlens,
+                                      int32_t* topk_pos, void* workspace, size_t workspace_bytes,
+                                      bgmoe_stream_t stream) {
+  BGMOE_REQUIRE(n >= 0 && k > 0, "token_sort_index: bad sizes n=%d k=%d", n, k);
+  BGMOE_REQUIRE(row_align > 0 && (row_align & (row_align - 1)) == 0,
+                "token_sort_index: row_align must be a positive power of two, got %d", row_align);
+  BGMOE_REQUIRE(num_local_experts > 0 && num_local_experts <= kMaxLocal,
+                "token_sort_index: num_local_experts=%d outside [1,%d]", num_local_experts, kMaxLocal);
+  BGMOE_REQUIRE(expert_start >= 0, "token_sort_index: expert_start out of range: %d", expert_start);
+  const int64_t nk = (int64_t)n * k;
+  BGMOE_REQUIRE(nk + (int64_t)(row_align - 1) * num_local_experts <= 2147483647LL,
+                "token_sort_index: N*K = %lld rows (padded to %d) exceed int32", (long long)nk, row_align);
+  BGMOE_REQUIRE(counts && cu_seqlens && (n == 0 || topk_pos), "token_sort_index: null output");
+  BGMOE_REQUIRE(n == 0 || topk_ids, "token_sort_index: null topk_ids");
+  PermArgs a{};
+  if (ids_are_int64) a.ids64 = (const int64_t*)topk_ids; else a.ids = (const int32_t*)topk_ids;
+  a.nk = nk; a.expert_start = expert_start; a.e_local = num_local_experts; a.mtp = 0; a.row_align = row_align;
+  a.counts = counts; a.counters = nullptr; a.cu = cu_seqlens; a.pos = topk_pos; a.extra_count = -1;
   return run_index(a, workspace, workspace_bytes, bgmoe_stream(stream));
 }
 

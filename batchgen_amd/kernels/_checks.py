@@ -58,3 +58,23 @@ def combine_args(expert_output, topk_pos, topk_weights, output, n, h, k, out_dty
 
 
 FP8_BYTES = (torch.uint8, torch.float8_e4m3fn)
+
+# BGMOE_DT_*: element types of the operators that take all three
+DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def dtype_code(t: torch.Tensor, name: str) -> int:
+    code = DTYPE_CODE.get(t.dtype)
+    if code is None:
+        fail(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
+    return code
+
+
+def rows_of(t: torch.Tensor, name: str) -> torch.Tensor:
+    """``t [..., K]`` as ``[rows, K]`` whose rows are contiguous (a 2-D tensor may keep a stride between its rows)."""
+    if t.dim() == 0:
+        fail(f"{name} must have at least one axis")
+    if t.dim() == 2 and (t.stride(1) == 1 or t.size(1) <= 1) and (t.stride(0) >= t.size(1) or t.size(0) <= 1):
+        return t
+    t2 = t.reshape(-1, t.size(-1)) if t.size(-1) else t.reshape(t.numel(), 0)
+    return t2 if t2.stride(1) == 1 and t2.stride(0) >= t2.size(1) else t2.contiguous()

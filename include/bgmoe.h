@@ -796,6 +796,110 @@ typedef struct bgmoe_moe_mxfp4_layer {
 
 int bgmoe_moe_mxfp4_layer_forward(const bgmoe_moe_mxfp4_layer* layer, int stages, bgmoe_stream_t stream);
 
+/* ------------------------------------------------ operators without a reference counterpart
+ * The three families below have no counterpart in the reference.  Element types of floating operands: */
+enum { BGMOE_DT_BF16 = 0, BGMOE_DT_FP16 = 1, BGMOE_DT_FP32 = 2 };
+
+/* -------------------------------------------------------- int8 products */
+
+/* One int8 scale per row: scale[r] = max(max_k |x[r][k]|, 1e-30) / 127 (IEEE fp32 division),
+ * q[r][k] = rint(x[r][k] / scale[r]) in [-127, 127] (ties to even).  A row that holds an infinity or a NaN gets a
+ * non-finite scale (and q = 0 where the quotient is NaN), so that a product over it is NaN instead of a number.
+ * x: element type `dtype`, rows x_row_stride elements apart; q [rows,k] contiguous. */
+int bgmoe_int8_quant_rows(const void* x, int dtype, int64_t x_row_stride, int64_t rows, int k, int8_t* q, float* scale,
+                          bgmoe_stream_t stream);
+
+/* out[t][j] = (sum_k x[t][k] * w[j][k]) * x_scale[t] * w_scale[j] (+ bias[j]): the sum is exact (int32 MFMA
+ * accumulators; k <= 131071), the two scalings and the bias are fp32, one rounding to out_dtype.  x [m,k] int8 with
+ * x_row_stride bytes between rows, w [n,k] int8 contiguous; k % 16 == 0, both 16-byte aligned, x_row_stride % 16 == 0.
+ * out rows are out_row_stride elements apart.  workspace: bgmoe_int8_gemm_workspace_bytes(m,n,k) bytes (0 = none
+ * needed): the int32 planes of a K split when m is small.  Results do not depend on the split. */
+size_t bgmoe_int8_gemm_workspace_bytes(int64_t m, int n, int k);
+int bgmoe_int8_gemm(const int8_t* x, int64_t x_row_stride, const float* x_scale, const int8_t* w, const float* w_scale,
+                    const float* bias, int64_t m, int n, int k, void* out, int out_dtype, int64_t out_row_stride,
+                    void* workspace, size_t workspace_bytes, bgmoe_stream_t stream);
+
+/* bgmoe_int8_quant_rows followed by bgmoe_int8_gemm in one call, with the same bits; the int8 rows and their scales
+ * live in the workspace (bgmoe_int8_linear_workspace_bytes(m,n,k) bytes, 16-byte aligned). */
+size_t bgmoe_int8_linear_workspace_bytes(int64_t m, int n, int k);
+int bgmoe_int8_linear(const void* x, int x_dtype, int64_t x_row_stride, const int8_t* w, const float* w_scale,
+                      const float* bias, int64_t m, int n, int k, void* out, int out_dtype, int64_t out_row_stride,
+                      void* workspace, size_t workspace_bytes, bgmoe_stream_t stream);
+
+/* The same product for rows grouped by expert: rows [cu_seqlens[g], cu_seqlens[g] + seqlens[g]) of x [m,k] times
+ * w[g] [n,k]; rows of no group are neither read nor written.  Group g's weights start w_group_stride bytes, its
+ * w_scale w_scale_group_stride floats after the previous group's (so gate and up may be halves of one stack).
+ * seqlens / cu_seqlens live on the device; counts that reach past m are cut there. */
+int bgmoe_int8_grouped_gemm(const int8_t* x, const float* x_scale, const int8_t* w, int64_t w_group_stride,
+                            const float* w_scale, int64_t w_scale_group_stride, const int32_t* seqlens,
+                            const int32_t* cu_seqlens, int groups, int64_t m, int n, int k, void* out, int out_dtype,
+                            bgmoe_stream_t stream);
+
+/* out = silu(gate) * up of two grouped products (fp32 in between, one rounding). */
+int bgmoe_int8_fused_s1(const int8_t* x, const float* x_scale, const int8_t* gate, int64_t gate_group_stride,
+                        const float* gate_scale, int64_t gate_scale_group_stride, const int8_t* up,
+                        int64_t up_group_stride, const float* up_scale, int64_t up_scale_group_stride,
+                        const int32_t* seqlens, const int32_t* cu_seqlens, int groups, int64_t m, int n, int k,
+                        void* out, int out_dtype, bgmoe_stream_t stream);
+
+/* ------------------------------------------- tokens sorted by expert and back */
+
+/* Where every (token, slot) pair goes: expert e owns rows [cu_seqlens[e], cu_seqlens[e] + counts[e]) in the stable
+ * (token, slot) order, cu_seqlens[e+1] - cu_seqlens[e] = counts[e] rounded up to row_align (a power of two);
+ * topk_pos[t*k+j] = the pair's row, -1 where topk_ids[t*k+j] - expert_start is outside [0, num_local_experts).
+ * topk_ids int32 or int64.  Same order as bgmoe_dispatch_scatter_ragged.  workspace: bgmoe_dispatch_workspace_bytes. */
+int bgmoe_token_sort_index(const void* topk_ids, int ids_are_int64, int n, int k, int expert_start,
+                           int num_local_experts, int row_align, int32_t* counts, int32_t* cu_seqlens,
+                           int32_t* topk_pos, void* workspace, size_t workspace_bytes, bgmoe_stream_t stream);
+
+/* out[topk_pos[t*k+j]] = x[t], bytes moved as they are (row_bytes per row; x rows x_row_stride bytes
+ * apart, out [rows,row_bytes] contiguous; any alignment).  zero_rest != 0 also clears the rows of out that
+ * hold no pair (padding of row_align, rows at or past cu_seqlens[num_local_experts]); otherwise they keep their bytes.
+ * k <= 32. */
+int bgmoe_token_sort_rows(const void* x, int64_t x_row_stride, int64_t row_bytes, int n, int k,
+                          const int32_t* topk_pos, const int32_t* counts, const int32_t* cu_seqlens,
+                          int num_local_experts, int64_t rows, int zero_rest, void* out, bgmoe_stream_t stream);
+
+/* out[t] = sum_j weights[t*k+j] * rows[topk_pos[t*k+j]] over the pairs with a row, j ascending, fp32 fused
+ * multiply-adds, one rounding (weights NULL: all 1).  Also the gradient of bgmoe_token_sort_rows (weights NULL). */
+int bgmoe_token_unsort(const void* rows, int dtype, const int32_t* topk_pos, const float* weights, int n, int k, int h,
+                       void* out, bgmoe_stream_t stream);
+
+/* Gradients of bgmoe_token_unsort: d_rows[topk_pos[t*k+j]] = weights[t*k+j] * d_out[t] (rows without a pair: 0),
+ * d_weights[t*k+j] = <d_out[t], rows[topk_pos[t*k+j]]> in fp32 (0 where the pair has no row).  Either output may be
+ * NULL.  No atomics: the same bits every time. */
+int bgmoe_token_unsort_backward(const void* d_out, const void* rows, int dtype, const int32_t* topk_pos,
+                                const float* weights, int n, int k, int h, const int32_t* counts,
+                                const int32_t* cu_seqlens, int num_local_experts, int64_t num_rows, void* d_rows,
+                                float* d_weights, bgmoe_stream_t stream);
+
+/* ----------------------------- norms before and after a block, gate, residual */
+
+/* p = RMSNorm(block) * post_weight (post_weight NULL: p = block); y = residual + residual_scale * gate * p;
+ * normed = RMSNorm(y) * pre_weight (pre_weight NULL: no normed), RMSNorm(v) = v / sqrt(mean(v^2) + eps).  fp32
+ * throughout: normed is taken from the unrounded y, each output is rounded once.  gate_mode: how gate is laid out.
+ * param_fp32: bit 0 / 1 / 2 set = post_weight / gate / pre_weight are fp32, else of type `dtype`.
+ * q / q_scale (optional, with pre_weight): bgmoe_int8_quant_rows of the stored normed, in the same pass.
+ * inv_post / inv_pre (optional, fp32 [rows]): 1 / sqrt(mean + eps) of the two norms, for the gradient.
+ * y may be the same memory as residual or block.  1 <= h <= 16384. */
+enum { BGMOE_GATE_NONE = 0, BGMOE_GATE_CHANNEL = 1 /* [h] */, BGMOE_GATE_TOKEN = 2 /* [rows] */, BGMOE_GATE_FULL = 3 /* [rows,h] */ };
+int bgmoe_gated_residual_norm(const void* block, const void* residual, int dtype, const void* post_weight,
+                              const void* gate, int gate_mode, float residual_scale, const void* pre_weight,
+                              int param_fp32, int64_t rows, int h, float eps, void* y, void* normed, int8_t* q,
+                              float* q_scale, float* inv_post, float* inv_pre, bgmoe_stream_t stream);
+
+/* Gradients of the above from d_y and d_normed (either may be NULL = zero): d_block, d_residual of type `dtype`,
+ * d_post / d_pre / d_gate of their operand's type (each may be NULL where not wanted).  inv_post / inv_pre as the
+ * forward pass stored them.  Sums over rows go through per-block fp32 planes in the workspace
+ * (bgmoe_gated_residual_norm_backward_workspace_bytes(rows, h)) and are added in a fixed order: no atomics. */
+size_t bgmoe_gated_residual_norm_backward_workspace_bytes(int64_t rows, int h);
+int bgmoe_gated_residual_norm_backward(const void* block, const void* residual, int dtype, const void* post_weight,
+                                       const void* gate, int gate_mode, float residual_scale, const void* pre_weight,
+                                       int param_fp32, int64_t rows, int h, const float* inv_post,
+                                       const float* inv_pre, const void* d_y, const void* d_normed, void* d_block,
+                                       void* d_residual, void* d_post, void* d_gate, void* d_pre, void* workspace,
+                                       size_t workspace_bytes, bgmoe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
