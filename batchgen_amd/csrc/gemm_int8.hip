@@ -209,13 +209,13 @@ __device__ __forceinline__ void stream_chunk(const Int8Args& a, uint8_t* smem, c
 }
 
 template <bool FUSED>
-__global__ __launch_bounds__(256) void int8_stream_kernel(Int8Args a) {
+__global__ __launch_bounds__(256) void int8_stream_kernel(Int8Args a, int max_rows) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int g = blockIdx.y;
   int64_t row0;
   int cnt;
   group_rows(a, g, &row0, &cnt);
-  if (cnt == 0) return;
+  if (cnt == 0 || cnt > max_rows) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = blockIdx.x * (FUSED ? 32 : 64);
   const bool second = FUSED && wave >= 2;
@@ -236,6 +236,211 @@ __global__ __launch_bounds__(256) void int8_stream_kernel(Int8Args a) {
     } else {
       stream_chunk<FUSED, 4>(a, smem, wbase, wrow0, wrows, ws, ws_up, row0, t0, cnt, n0);
       t0 += 64;
+    }
+  }
+}
+
+// ---- tiled kernel: many rows per group ---------------------------------------------------------------------------------
+// Macro tile 256 tokens x 256 weight rows (fused: 128 gate + 128 up), 8 waves = 4 (64 weight rows) x 2 (128 tokens); a wave
+// holds 2 x 4 tiles of v_mfma_i32_32x32x32_i8, 128 accumulators.  K advances 64 bytes per step through a ring of four
+// 32 KB slots.  One barrier per step, in its middle:
+//
+//   read the step's second half of the operands | 8 MFMAs of the first half | wait for the next step's loads, barrier
+//   request step s + 4 into this step's slot | read the next step's first half | 8 MFMAs of the second half
+//
+// so that each batch of LDS reads runs under the MFMAs of the batch before it, a slot is requested again as soon as
+// the barrier says that every wave has read it, and up to three steps (96 KB per CU) are in flight from L2 and HBM.
+// A row's four 16-byte chunks of a step lie at chunk ^ ((row / 4) & 3): the 16 lanes that read one chunk of 16 rows hit
+// 16 different 16-byte slots of 256 bytes.
+constexpr int kTM = 256, kTW = 256, kTK = 64, kSlots = 4;
+constexpr int kSlotBytes = (kTM + kTW) * kTK;
+constexpr int kMaxGroups = 1024;
+constexpr int kPanel = 8;                     // m-tiles that share their weight tiles in an XCD's L2
+
+template <bool FUSED>
+__global__ __launch_bounds__(512) void int8_tiled_kernel(Int8Args a, int groups, int min_rows) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int s_tiles[kMaxGroups + 1];
+  constexpr int kCols = FUSED ? 128 : 256;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave & 3, wm = wave >> 2;
+  const int ntn = (a.n + kCols - 1) / kCols;
+
+  // ---- which (group, m-tile, n-tile): block b runs on XCD b % 8 and takes items of that eighth of the list ----
+  int total_m;
+  if (a.seqlens == nullptr) {
+    total_m = (int)((a.m + kTM - 1) / kTM);
+  } else {
+    if (tid < 64) {                           // one wave scans the groups' tile counts
+      int run = 0;
+      for (int g0 = 0; g0 < groups; g0 += 64) {
+        const int g = g0 + lane;
+        int64_t r0;
+        int c = 0;
+        if (g < groups) group_rows(a, g, &r0, &c);
+        const int t = c > min_rows ? (c + kTM - 1) / kTM : 0;
+        int inc = t;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          const int up = __shfl_up(inc, off, BGMOE_WAVE);
+          if (lane >= off) inc += up;
+        }
+        if (g < groups) s_tiles[g + 1] = run + inc;
+        run += __shfl(inc, 63, BGMOE_WAVE);
+      }
+      if (lane == 0) s_tiles[0] = 0;
+    }
+    __syncthreads();
+    total_m = s_tiles[groups];
+  }
+  const int64_t total = (int64_t)total_m * ntn;
+  const int64_t per_x = (total + 7) / 8;
+  const int64_t idx = blockIdx.x >> 3;
+  const int64_t item = (int64_t)(blockIdx.x & 7) * per_x + idx;
+  if (idx >= per_x || item >= total) return;
+  int grp = 0, m_tiles = total_m, first = 0;
+  if (a.seqlens != nullptr) {
+    int lo = 0, hi = groups - 1;              // the last group whose tiles start at or before the item
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((int64_t)s_tiles[mid] * ntn <= item) lo = mid;
+      else hi = mid - 1;
+    }
+    grp = __builtin_amdgcn_readfirstlane(lo);
+    first = __builtin_amdgcn_readfirstlane(s_tiles[grp]);
+    m_tiles = __builtin_amdgcn_readfirstlane(s_tiles[grp + 1]) - first;
+  }
+  const int64_t rel = item - (int64_t)first * ntn;
+  const int panel = (int)(rel / ((int64_t)kPanel * ntn));
+  const int pm = min(kPanel, m_tiles - panel * kPanel);
+  const int in_panel = (int)(rel - (int64_t)panel * kPanel * ntn);
+  const int nt = in_panel / pm;
+  const int m0 = (panel * kPanel + in_panel - nt * pm) * kTM, n0 = nt * kCols;
+  int64_t row0;
+  int cnt;
+  group_rows(a, grp, &row0, &cnt);
+
+  // ---- load sources: wave load i of this wave covers 16 rows x 64 bytes; lane = row lane / 4, LDS position lane % 4 ----
+  const int lr = lane >> 2, lc = (lane & 3) ^ ((lane >> 4) & 3);
+  const uint8_t* xsrc = uniform_ptr(reinterpret_cast<const uint8_t*>(a.x) + (row0 + m0) * a.ldx);
+  const uint8_t* wsrc[2];
+  uint32_t x_off[2], w_off[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 16 * (2 * wave + i);
+    x_off[i] = (uint32_t)min(r + lr, cnt - 1 - m0) * (uint32_t)a.ldx + (uint32_t)(lc * 16);
+    const bool up = FUSED && r >= 128;
+    const int8_t* base = up ? a.w1 + grp * a.w1_group : a.w0 + grp * a.w0_group;
+    const int first_row = min(n0 + (FUSED ? r & 127 : r), a.n - 1);
+    wsrc[i] = uniform_ptr(reinterpret_cast<const uint8_t*>(base) + (int64_t)first_row * a.k);
+    w_off[i] = (uint32_t)min(lr, a.n - 1 - first_row) * (uint32_t)a.k + (uint32_t)(lc * 16);
+  }
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
+  const int S = (a.k + kTK - 1) / kTK;
+  const int chunks = a.k >> 4;
+  auto issue = [&](int s) {
+    const uint32_t d = lds0 + (uint32_t)(s & (kSlots - 1)) * kSlotBytes + 2048 * wave;
+    const int ko = s * kTK;
+    if ((s + 1) * 4 <= chunks) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) async_load16(xsrc + ko, x_off[i], d + i * 1024);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) async_load16(wsrc[i] + ko, w_off[i], d + kTM * kTK + i * 1024);
+    } else {                                  // the last, partial step: chunks past K read zeros
+      const bool in = s * 4 + lc < chunks;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        async_load16_lane(in ? (const void*)(xsrc + ko + x_off[i]) : (const void*)&g_zeros, d + i * 1024);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        async_load16_lane(in ? (const void*)(wsrc[i] + ko + w_off[i]) : (const void*)&g_zeros, d + kTM * kTK + i * 1024);
+    }
+  };
+
+  // ---- operand reads: 32 rows x 32 bytes of K per tile; lane = row lane % 32, chunk 2 h + lane / 32 ----
+  const int fr = lane & 31, fq = lane >> 5;
+  const int sw = (fr >> 2) & 3;
+  const int f_off[2] = {fr * kTK + ((fq ^ sw) * 16), fr * kTK + (((2 + fq) ^ sw) * 16)};
+  int a_off[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) a_off[i] = kTM * kTK + 32 * kTK * (FUSED ? 4 * i + wn : 2 * wn + i);
+  const int b_off = 128 * kTK * wm;
+  struct Frag { intx4 w[2], x[4]; };
+  auto read = [&](int s, int h, Frag& f) {
+    const uint8_t* b = smem + (s & (kSlots - 1)) * kSlotBytes;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) f.w[i] = *reinterpret_cast<const intx4*>(b + a_off[i] + f_off[h]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.x[j] = *reinterpret_cast<const intx4*>(b + b_off + 32 * kTK * j + f_off[h]);
+  };
+  intx16 acc[2][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
+  auto multiply = [&](const Frag& f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[i], f.x[j], acc[i][j], 0, 0, 0);
+  };
+
+  for (int s = 0; s < kSlots && s < S; ++s) issue(s);
+  if (S >= kSlots) wait_vm<4 * (kSlots - 1)>();
+  else wait_vm<0>();
+  block_barrier();
+  Frag f0, f1;
+  read(0, 0, f0);
+  for (int s = 0; s < S; ++s) {
+    read(s, 1, f1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(f0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (s + 1 < S) {
+      if (s + 3 < S) wait_vm<8>();            // steps s + 2 and s + 3 may still be in flight
+      else wait_vm<0>();
+      lds_exchange_barrier();                 // step s + 1 is there; everybody has read step s
+      if (s + kSlots < S) issue(s + kSlots);
+      read(s + 1, 0, f0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(f1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // ---- epilogue: lane holds, for token lane % 32 of each token tile, columns 8 b + 4 (lane / 32) + 0..3, b = 0..3 ----
+  const float* ws0 = a.ws0 + grp * a.ws0_group;
+  const float* ws1 = FUSED ? a.ws1 + grp * a.ws1_group : nullptr;
+#pragma unroll
+  for (int i = 0; i < (FUSED ? 1 : 2); ++i) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int col = n0 + (FUSED ? 32 * wn : 64 * wn + 32 * i) + 8 * b + 4 * fq;
+      float sc[4], su[4], bias[4];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int c = min(col + v, a.n - 1);
+        sc[v] = ws0[c];
+        su[v] = FUSED ? ws1[c] : 0.0f;
+        bias[v] = a.bias ? a.bias[c] : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int tok = m0 + 128 * wm + 32 * j + fr;
+        if (tok >= cnt) continue;
+        const float xs = a.xs[row0 + tok];
+        float v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          v[u] = (float)acc[i][j][4 * b + u] * xs * sc[u];
+          if constexpr (FUSED) v[u] = silu_f32(v[u]) * ((float)acc[1][j][4 * b + u] * xs * su[u]);
+          else if (a.bias) v[u] += bias[u];
+        }
+        store4(a, row0 + tok, col, v);
+      }
     }
   }
 }
@@ -320,24 +525,42 @@ int check_sizes(const char* what, int64_t m, int n, int k, int out_dtype) {
   return BGMOE_OK;
 }
 
+// Groups of up to kStreamRows rows are streamed, larger ones tiled; each kernel skips the other's groups.
+constexpr int kStreamRows = 64;
+
 int run_gemm(const char* what, const Int8Args& a, int groups, hipStream_t st) {
   const bool fused = a.w1 != nullptr;
   const int cols = fused ? 32 : 64;
   const int64_t tiles = ((int64_t)a.n + cols - 1) / cols;
   BGMOE_REQUIRE(tiles <= 1 << 24, "%s: n=%d is too wide", what, a.n);
-  const dim3 grid((unsigned)tiles, (unsigned)groups), block(256);
+  const bool grouped = a.seqlens != nullptr;
   BgmoeProf prof(BGMOE_K_INT8_GEMM, st);
-  if (fused) hipLaunchKernelGGL(int8_stream_kernel<true>, grid, block, kRingBytes, st, a);
-  else hipLaunchKernelGGL(int8_stream_kernel<false>, grid, block, kRingBytes, st, a);
+  if (grouped || a.m <= kStreamRows) {
+    const dim3 grid((unsigned)tiles, (unsigned)groups), block(256);
+    if (fused) hipLaunchKernelGGL(int8_stream_kernel<true>, grid, block, kRingBytes, st, a, kStreamRows);
+    else hipLaunchKernelGGL(int8_stream_kernel<false>, grid, block, kRingBytes, st, a, kStreamRows);
+  }
+  if (a.m > kStreamRows) {                    // a bound on the m-tiles of groups above the limit, whatever the counts
+    const int64_t m_tiles = grouped ? a.m / kTM + min((int64_t)groups, a.m / (kStreamRows + 1)) : (a.m + kTM - 1) / kTM;
+    const int64_t items = m_tiles * ((a.n + (fused ? 127 : 255)) / (fused ? 128 : 256));
+    const int64_t blocks = (items + 7) / 8 * 8;
+    BGMOE_REQUIRE(blocks <= 1 << 22, "%s: m=%lld x n=%d is too large for one launch", what, (long long)a.m, a.n);
+    const dim3 grid((unsigned)blocks), block(512);
+    if (fused) hipLaunchKernelGGL(int8_tiled_kernel<true>, grid, block, kSlots * kSlotBytes, st, a, groups, kStreamRows);
+    else hipLaunchKernelGGL(int8_tiled_kernel<false>, grid, block, kSlots * kSlotBytes, st, a, groups, kStreamRows);
+  }
   return bgmoe_check_launch(what);
 }
 
 }  // namespace
 
 int bgmoe_internal_init_int8_gemm() {
-  const void* fns[2] = {(const void*)int8_stream_kernel<false>, (const void*)int8_stream_kernel<true>};
-  for (const void* f : fns) {
-    const hipError_t err = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+  const struct { const void* fn; int bytes; } fns[4] = {{(const void*)int8_stream_kernel<false>, kRingBytes},
+                                                        {(const void*)int8_stream_kernel<true>, kRingBytes},
+                                                        {(const void*)int8_tiled_kernel<false>, kSlots * kSlotBytes},
+                                                        {(const void*)int8_tiled_kernel<true>, kSlots * kSlotBytes}};
+  for (const auto& f : fns) {
+    const hipError_t err = hipFuncSetAttribute(f.fn, hipFuncAttributeMaxDynamicSharedMemorySize, f.bytes);
     if (err != hipSuccess) {
       bgmoe_set_error("int8 product: hipFuncSetAttribute(dynamic LDS) failed: %s", hipGetErrorString(err));
       return BGMOE_ERR_HIP;
@@ -387,7 +610,7 @@ extern "C" int bgmoe_int8_gemm(const int8_t* x, int64_t x_row_stride, const floa
   BGMOE_REQUIRE(x && x_scale && w && w_scale && out, "int8_gemm: null pointer");
   BGMOE_REQUIRE(((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_row_stride) % 16 == 0,
                 "int8_gemm: x, w and x_row_stride must be multiples of 16 bytes");
-  BGMOE_REQUIRE(x_row_stride >= k && x_row_stride < (1LL << 25), "int8_gemm: x_row_stride %lld outside [k, 2^25)",
+  BGMOE_REQUIRE(x_row_stride >= k && x_row_stride < (1LL << 24), "int8_gemm: x_row_stride %lld outside [k, 2^24)",
                 (long long)x_row_stride);
   BGMOE_REQUIRE(out_row_stride >= n, "int8_gemm: out_row_stride %lld is smaller than n=%d", (long long)out_row_stride, n);
   (void)workspace; (void)workspace_bytes;
@@ -433,7 +656,7 @@ extern "C" int bgmoe_int8_linear(const void* x, int x_dtype, int64_t x_row_strid
 static int grouped(const char* what, Int8Args& a, int groups, int out_dtype, bgmoe_stream_t stream) {
   int rc = check_sizes(what, a.m, a.n, a.k, out_dtype);
   if (rc != BGMOE_OK) return rc;
-  BGMOE_REQUIRE(groups >= 1 && groups <= 65535, "%s: %d groups outside [1, 65535]", what, groups);
+  BGMOE_REQUIRE(groups >= 1 && groups <= kMaxGroups, "%s: %d groups outside [1, %d]", what, groups, kMaxGroups);
   if (a.m == 0 || a.n == 0) return BGMOE_OK;
   BGMOE_REQUIRE(a.x && a.xs && a.w0 && a.ws0 && a.seqlens && a.cu && a.out, "%s: null pointer", what);
   BGMOE_REQUIRE(((uintptr_t)a.x | (uintptr_t)a.w0 | (uintptr_t)a.w0_group | (uintptr_t)a.w1 | (uintptr_t)a.w1_group) % 16 == 0,

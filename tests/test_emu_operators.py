@@ -130,3 +130,31 @@ def test_int8_refusals():
     refused(f, P, P, P, 520, P, 8, P, P, 1, 4, 8, 64, P, 0, None, says="16 bytes")
     refused(f, P, P, P, 512, P, 8, None, P, 1, 4, 8, 64, P, 0, None, says="null pointer")
     refused("bgmoe_int8_fused_s1", P, P, P, 512, P, 8, None, 512, P, 8, P, P, 1, 4, 8, 64, P, 0, None, says="null pointer")
+
+
+@pytest.mark.parametrize("mode", [1, 2], ids=["loads land late", "loads land late, ordinary loads counted"])
+@pytest.mark.parametrize("schedule", [0, 1, 2])
+@pytest.mark.parametrize("m,n,k", [(5, 70, 1296), (33, 64, 800), (70, 40, 64), (200, 130, 656), (300, 300, 144)])
+def test_int8_rings_wait_for_what_they_read(mode, schedule, m, n, k):
+    """The asynchronous loads landing as late as the kernels' own waits allow, with the largest skew between waves that
+    the barriers allow, in guarded buffers: a wait that is too lenient gives wrong sums, an access out of range ends the
+    test process with a message."""
+    import numpy as np
+    from tests import emu
+    h = emu.load()
+    rng = np.random.default_rng(m + k)
+    x, w = (emu.guarded(rng.integers(-128, 128, s, dtype=np.int8)) for s in ((m, k), (n, k)))
+    xs, ws = (emu.guarded(rng.uniform(0.5, 1.5, s).astype(np.float32)) for s in (m, n))
+    out = emu.guarded(np.zeros((m, n), np.float32))
+    need = h.bgmoe_int8_gemm_workspace_bytes(m, n, k)
+    work = emu.guarded(np.full(max(need, 1), 255, np.uint8))
+    h.emu_set_async_mode(mode)
+    h.emu_set_schedule(schedule)
+    try:
+        emu.ok(h, h.bgmoe_int8_gemm(emu.p(x), k, emu.p(xs), emu.p(w), emu.p(ws), None, m, n, k, emu.p(out), 2, n, emu.p(work),
+                                    need, None))
+    finally:
+        h.emu_set_async_mode(0)
+        h.emu_set_schedule(0)
+    want = (x.astype(np.int64) @ w.astype(np.int64).T).astype(np.float32) * xs[:, None] * ws[None, :]
+    assert np.array_equal(out, want)
