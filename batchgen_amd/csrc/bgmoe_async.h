@@ -41,6 +41,12 @@ __device__ __forceinline__ const T* uniform_ptr(const T* p) {   // tell the comp
 template <int N>
 __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 __device__ __forceinline__ void block_barrier() { asm volatile("s_barrier" ::: "memory"); }
+// This wave's LDS reads have returned.  Unlike an inline-asm wait the compiler counts this one: it places no wait of its
+// own before the registers' first use, which would also wait for younger reads.
+__device__ __forceinline__ void lds_reads_done() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);           // lgkmcnt(0), the other counters at their maximum
+  asm volatile("" ::: "memory");
+}
 // Barrier for an exchange through LDS only: this wave's LDS writes are done (lgkmcnt(0)), then the barrier.  Unlike
 // __syncthreads() it does not wait for vector-memory operations, so asynchronous global -> LDS loads that are in
 // flight for LATER use stay in flight across it.

@@ -242,20 +242,88 @@ __global__ __launch_bounds__(256) void int8_stream_kernel(Int8Args a, int max_ro
 
 // ---- tiled kernel: many rows per group ---------------------------------------------------------------------------------
 // Macro tile 256 tokens x 256 weight rows (fused: 128 gate + 128 up), 8 waves = 4 (64 weight rows) x 2 (128 tokens); a wave
-// holds 2 x 4 tiles of v_mfma_i32_32x32x32_i8, 128 accumulators.  K advances 64 bytes per step through a ring of four
-// 32 KB slots.  One barrier per step, in its middle:
+// holds 4 x 8 tiles of v_mfma_i32_16x16x64_i8, 128 accumulators.  K advances 128 bytes per step through two 64 KB slots.
+// Whole 128-byte lines on purpose: a CU takes in 134 GB/s through asynchronous loads whose lanes cover 128-byte pieces of
+// rows, 65 GB/s with 64-byte pieces, however many are in flight; a step needs 64 KB in the 0.9 us its MFMAs take.
+// A step is two halves of 64 bytes.  While a half is multiplied the operands of the next one are read from LDS, and in
+// the second half the step after next is requested; both are spread between the MFMAs, two reads and one load per
+// four (all of them behind the barrier: 20% more time per step with 16 CUs at work, since 64 loads keep the CU's address
+// unit busy for as long as half the step's MFMAs).  One barrier per step:
 //
-//   read the step's second half of the operands | 8 MFMAs of the first half | wait for the next step's loads, barrier
-//   request step s + 4 into this step's slot | read the next step's first half | 8 MFMAs of the second half
+//   multiply half 0, read half 1 | wait for the next step's loads and this wave's reads, barrier: the next step is there,
+//   this slot is free | multiply half 1, read the next step's half 0, request step s + 2 into this slot
 //
-// so that each batch of LDS reads runs under the MFMAs of the batch before it, a slot is requested again as soon as
-// the barrier says that every wave has read it, and up to three steps (96 KB per CU) are in flight from L2 and HBM.
-// A row's four 16-byte chunks of a step lie at chunk ^ ((row / 4) & 3): the 16 lanes that read one chunk of 16 rows hit
-// 16 different 16-byte slots of 256 bytes.
-constexpr int kTM = 256, kTW = 256, kTK = 64, kSlots = 4;
+// A row's eight 16-byte chunks of a step lie at chunk ^ ((row / 2) & 7): the 16 lanes that read one chunk of 16 rows hit
+// 16 different 16-byte slots of 256 bytes (no bank conflicts by the counter).
+// Bound: the chip's power.  With every CU at work the MFMAs alone run at 3.2 (32x32x32) and 3.6 (16x16x64) PFLOP/s on
+// normally distributed bytes, because the clock falls to about 1.6 GHz; this loop runs at 2.7.
+constexpr int kTM = 256, kTW = 256, kTK = 128, kSlots = 2;
 constexpr int kSlotBytes = (kTM + kTW) * kTK;
 constexpr int kMaxGroups = 1024;
 constexpr int kPanel = 8;                     // m-tiles that share their weight tiles in an XCD's L2
+
+// four consecutive per-column values, the last one repeated past n
+__device__ __forceinline__ void load_cols(const float* p, int col, int n, float (&v)[4]) {
+  if (col + 3 < n) {
+    const u32x4 r = load16(p + col);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = p[min(col + i, n - 1)];
+  }
+}
+// Writes a wave's 128 tokens x 16 TILES columns: value(i, j, v) gives the lane's four columns of column tile i and token
+// tile j.  A row of the patch is one token's columns in 16-byte chunks at chunk ^ (row mod chunks per row).
+template <typename T, int TILES, typename V>
+__device__ __forceinline__ void store_tiles(const Int8Args& a, uint8_t* patch, int64_t row0, int rows, int wcol, V value) {
+  constexpr int kChunks = TILES * T::kBytes;           // 16-byte chunks per row
+  constexpr int kPer = 16 / T::kBytes;                 // columns per chunk
+  const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (16 * j >= rows) break;                         // wave-uniform
+    uint8_t* buf = patch + (j & 1) * 4096;             // two patches: the next tile is written while this one leaves
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) {
+      float v[4];
+      value(i, j, v);
+      uint8_t* row = buf + fr * kChunks * 16;
+      if constexpr (T::kBytes == 4) {
+        const u32x4 w = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+        *reinterpret_cast<u32x4*>(row + ((4 * i + fq) ^ (fr & (kChunks - 1))) * 16) = w;
+      } else {
+        const float w[8] = {v[0], v[1], v[2], v[3], 0.0f, 0.0f, 0.0f, 0.0f};
+        const u32x4 packed = pack16<T>(w);
+        *reinterpret_cast<uint2*>(row + ((2 * i + (fq >> 1)) ^ (fr & (kChunks - 1))) * 16 + (fq & 1) * 8) =
+            make_uint2(packed[0], packed[1]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int t = 0; t < kChunks / 4; ++t) {
+      const int idx = t * 64 + lane, row = idx / kChunks, c = idx % kChunks;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(buf + row * kChunks * 16 + (c ^ (row & (kChunks - 1))) * 16);
+      const int left = a.n - (wcol + c * kPer);
+      if (16 * j + row < rows && left > 0) {
+        uint8_t* dst = a.out + ((row0 + 16 * j + row) * a.ldo + wcol + c * kPer) * T::kBytes;
+        if (left >= kPer) {
+          store16(dst, v);
+        } else {
+          for (int u = 0; u < left; ++u) {
+            if constexpr (T::kBytes == 4) reinterpret_cast<uint32_t*>(dst)[u] = v[u];
+            else reinterpret_cast<uint16_t*>(dst)[u] = (uint16_t)(v[u >> 1] >> (16 * (u & 1)));
+          }
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 
 template <bool FUSED>
 __global__ __launch_bounds__(512) void int8_tiled_kernel(Int8Args a, int groups, int min_rows) {
@@ -321,128 +389,152 @@ __global__ __launch_bounds__(512) void int8_tiled_kernel(Int8Args a, int groups,
   int cnt;
   group_rows(a, grp, &row0, &cnt);
 
-  // ---- load sources: wave load i of this wave covers 16 rows x 64 bytes; lane = row lane / 4, LDS position lane % 4 ----
-  const int lr = lane >> 2, lc = (lane & 3) ^ ((lane >> 4) & 3);
+  // ---- load sources: a wave load covers 8 rows x 128 bytes; lane = row lane / 8, LDS position lane % 8.  This wave
+  // loads token rows and weight rows 32 wave .. 32 wave + 31 of the tile, four loads each ----
+  const int lr = lane >> 3;
+  const int lc[2] = {(lane & 7) ^ (lane >> 4), (lane & 7) ^ (4 + (lane >> 4))};      // source chunk in even and odd loads
   const uint8_t* xsrc = uniform_ptr(reinterpret_cast<const uint8_t*>(a.x) + (row0 + m0) * a.ldx);
-  const uint8_t* wsrc[2];
-  uint32_t x_off[2], w_off[2];
+  const bool up = FUSED && wave >= 4;
+  const int8_t* wmat = up ? a.w1 + grp * a.w1_group : a.w0 + grp * a.w0_group;
+  const int first_row = min(n0 + (FUSED ? 32 * (wave & 3) : 32 * wave), a.n - 1);
+  const uint8_t* wsrc = uniform_ptr(reinterpret_cast<const uint8_t*>(wmat) + (int64_t)first_row * a.k);
+  uint32_t x_off[4], w_off[4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = 16 * (2 * wave + i);
-    x_off[i] = (uint32_t)min(r + lr, cnt - 1 - m0) * (uint32_t)a.ldx + (uint32_t)(lc * 16);
-    const bool up = FUSED && r >= 128;
-    const int8_t* base = up ? a.w1 + grp * a.w1_group : a.w0 + grp * a.w0_group;
-    const int first_row = min(n0 + (FUSED ? r & 127 : r), a.n - 1);
-    wsrc[i] = uniform_ptr(reinterpret_cast<const uint8_t*>(base) + (int64_t)first_row * a.k);
-    w_off[i] = (uint32_t)min(lr, a.n - 1 - first_row) * (uint32_t)a.k + (uint32_t)(lc * 16);
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + lr;
+    x_off[i] = (uint32_t)min(32 * wave + r, cnt - 1 - m0) * (uint32_t)a.ldx + (uint32_t)(lc[i & 1] * 16);
+    w_off[i] = (uint32_t)min(r, a.n - 1 - first_row) * (uint32_t)a.k + (uint32_t)(lc[i & 1] * 16);
   }
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
-  const int S = (a.k + kTK - 1) / kTK;
+  const int S = max((a.k + kTK - 1) / kTK, 3);        // a short K is padded with steps of zeros
   const int chunks = a.k >> 4;
+  auto issue_one = [&](int s, int i) {        // one of the eight loads of a whole step
+    const uint32_t d = lds0 + (uint32_t)(s & 1) * kSlotBytes + 4096 * wave + (i & 3) * 1024;
+    if (i < 4) async_load16(xsrc + s * kTK, x_off[i & 3], d);
+    else async_load16(wsrc + s * kTK, w_off[i & 3], d + kTM * kTK);
+  };
   auto issue = [&](int s) {
-    const uint32_t d = lds0 + (uint32_t)(s & (kSlots - 1)) * kSlotBytes + 2048 * wave;
+    if ((s + 1) * 8 <= chunks) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) issue_one(s, i);
+      return;
+    }
+    const uint32_t d = lds0 + (uint32_t)(s & 1) * kSlotBytes + 4096 * wave;
     const int ko = s * kTK;
-    if ((s + 1) * 4 <= chunks) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) async_load16(xsrc + ko, x_off[i], d + i * 1024);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) async_load16(wsrc[i] + ko, w_off[i], d + kTM * kTK + i * 1024);
-    } else {                                  // the last, partial step: chunks past K read zeros
-      const bool in = s * 4 + lc < chunks;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        async_load16_lane(in ? (const void*)(xsrc + ko + x_off[i]) : (const void*)&g_zeros, d + i * 1024);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        async_load16_lane(in ? (const void*)(wsrc[i] + ko + w_off[i]) : (const void*)&g_zeros, d + kTM * kTK + i * 1024);
+    for (int i = 0; i < 4; ++i) {             // the last, partial step: chunks past K read zeros
+      const bool in = s * 8 + lc[i & 1] < chunks;
+      async_load16_lane(in ? (const void*)(xsrc + ko + x_off[i]) : (const void*)&g_zeros, d + i * 1024);
+      async_load16_lane(in ? (const void*)(wsrc + ko + w_off[i]) : (const void*)&g_zeros, d + kTM * kTK + i * 1024);
     }
   };
 
-  // ---- operand reads: 32 rows x 32 bytes of K per tile; lane = row lane % 32, chunk 2 h + lane / 32 ----
-  const int fr = lane & 31, fq = lane >> 5;
-  const int sw = (fr >> 2) & 3;
-  const int f_off[2] = {fr * kTK + ((fq ^ sw) * 16), fr * kTK + (((2 + fq) ^ sw) * 16)};
-  int a_off[2];
+  // ---- operands: 16 rows x 64 bytes of K per tile; lane = row lane % 16, chunk 4 half + lane / 16 ----
+  const int fr = lane & 15, fq = lane >> 4;
+  int f_off[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) a_off[i] = kTM * kTK + 32 * kTK * (FUSED ? 4 * i + wn : 2 * wn + i);
+  for (int h = 0; h < 2; ++h) f_off[h] = fr * kTK + (((4 * h + fq) ^ ((fr >> 1) & 7)) * 16);
+  int a_off[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a_off[i] = kTM * kTK + 16 * kTK * (FUSED ? 8 * (i >> 1) + 2 * wn + (i & 1) : 4 * wn + i);
   const int b_off = 128 * kTK * wm;
-  struct Frag { intx4 w[2], x[4]; };
-  auto read = [&](int s, int h, Frag& f) {
-    const uint8_t* b = smem + (s & (kSlots - 1)) * kSlotBytes;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) f.w[i] = *reinterpret_cast<const intx4*>(b + a_off[i] + f_off[h]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) f.x[j] = *reinterpret_cast<const intx4*>(b + b_off + 32 * kTK * j + f_off[h]);
+  // the weights of a half are double-buffered; a token tile's register is refilled as soon as it has been multiplied
+  intx4 w0[4], w1[4], x[8];
+  auto read_w = [&](int s, int h, int i) {
+    return *reinterpret_cast<const intx4*>(smem + (s & 1) * kSlotBytes + f_off[h] + a_off[i]);
   };
-  intx16 acc[2][4];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
-  auto multiply = [&](const Frag& f) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[i], f.x[j], acc[i][j], 0, 0, 0);
+  auto read_x = [&](int s, int h, int j) {
+    return *reinterpret_cast<const intx4*>(smem + (s & 1) * kSlotBytes + f_off[h] + b_off + 16 * kTK * j);
   };
-
-  for (int s = 0; s < kSlots && s < S; ++s) issue(s);
-  if (S >= kSlots) wait_vm<4 * (kSlots - 1)>();
-  else wait_vm<0>();
-  block_barrier();
-  Frag f0, f1;
-  read(0, 0, f0);
-  for (int s = 0; s < S; ++s) {
-    read(s, 1, f1);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(f0);
-    __builtin_amdgcn_sched_barrier(0);
-    if (s + 1 < S) {
-      if (s + 3 < S) wait_vm<8>();            // steps s + 2 and s + 3 may still be in flight
-      else wait_vm<0>();
-      lds_exchange_barrier();                 // step s + 1 is there; everybody has read step s
-      if (s + kSlots < S) issue(s + kSlots);
-      read(s + 1, 0, f0);
+  intx4 acc[4][8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = intx4{0, 0, 0, 0};
+  // multiplies w with x while reading half rh of step rs into wn and x; LOAD: requests step ls
+  auto half = [&](auto load, const intx4 (&w)[4], intx4 (&wnext)[4], int rs, int rh, int ls) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (decltype(load)::value) issue_one(ls, j);
+      if (j < 4) wnext[j] = read_w(rs, rh, j);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], x[j], acc[i][j], 0, 0, 0);
+      x[j] = read_x(rs, rh, j);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(f1);
-    __builtin_amdgcn_sched_barrier(0);
-  }
+  };
 
-  // ---- epilogue: lane holds, for token lane % 32 of each token tile, columns 8 b + 4 (lane / 32) + 0..3, b = 0..3 ----
+  issue(0);
+  issue(1);
+  wait_vm<8>();
+  block_barrier();
+  // a wave without a row of either operand inside the problem only loads and keeps the barriers
+  const bool live = m0 + 128 * wm < cnt && n0 + (FUSED ? 32 : 64) * wn < a.n;
+  if (!live) {
+    for (int s = 0; s + 1 < S; ++s) {
+      wait_vm<0>();
+      block_barrier();
+      if (s + 2 < S) issue(s + 2);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w0[i] = read_w(0, 0, i);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = read_x(0, 0, j);
+  auto next_step = [&] {                      // step s + 1 is there; everybody has read step s
+    wait_vm<0>();
+    lds_reads_done();
+    block_barrier();
+  };
+  for (int s = 0; s < S - 3; ++s) {
+    half(No{}, w0, w1, s, 1, 0);
+    next_step();
+    half(Yes{}, w1, w0, s + 1, 0, s + 2);     // step s + 2 < S - 1 is whole
+  }
+  // the last three steps, without a loop (one behind the other would make the compiler move accumulators around)
+  half(No{}, w0, w1, S - 3, 1, 0);
+  next_step();
+  issue(S - 1);
+  half(No{}, w1, w0, S - 2, 0, 0);
+  half(No{}, w0, w1, S - 2, 1, 0);
+  next_step();
+  half(No{}, w1, w0, S - 1, 0, 0);
+  half(No{}, w0, w1, S - 1, 1, 0);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w1[i], x[j], acc[i][j], 0, 0, 0);
+
+  // ---- epilogue: a lane holds columns 4 q .. 4 q + 3 of each 16-column tile for token r of each token tile ----
+  constexpr int kTiles = FUSED ? 2 : 4;       // 16-column tiles of the output
   const float* ws0 = a.ws0 + grp * a.ws0_group;
   const float* ws1 = FUSED ? a.ws1 + grp * a.ws1_group : nullptr;
+  const int wcol = n0 + 16 * kTiles * wn;     // this wave's first column
+  float sc[4][4], bias[kTiles][4], xs[8];
 #pragma unroll
-  for (int i = 0; i < (FUSED ? 1 : 2); ++i) {
+  for (int j = 0; j < 8; ++j) xs[j] = a.xs[row0 + min(m0 + 128 * wm + 16 * j + fr, cnt - 1)];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int col = n0 + (FUSED ? 32 * wn : 64 * wn + 32 * i) + 8 * b + 4 * fq;
-      float sc[4], su[4], bias[4];
+  for (int i = 0; i < 4; ++i) load_cols(i < kTiles ? ws0 : ws1, wcol + 16 * (i % kTiles) + 4 * fq, a.n, sc[i]);
+  if (a.bias) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int c = min(col + v, a.n - 1);
-        sc[v] = ws0[c];
-        su[v] = FUSED ? ws1[c] : 0.0f;
-        bias[v] = a.bias ? a.bias[c] : 0.0f;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int tok = m0 + 128 * wm + 32 * j + fr;
-        if (tok >= cnt) continue;
-        const float xs = a.xs[row0 + tok];
-        float v[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          v[u] = (float)acc[i][j][4 * b + u] * xs * sc[u];
-          if constexpr (FUSED) v[u] = silu_f32(v[u]) * ((float)acc[1][j][4 * b + u] * xs * su[u]);
-          else if (a.bias) v[u] += bias[u];
-        }
-        store4(a, row0 + tok, col, v);
-      }
-    }
+    for (int i = 0; i < kTiles; ++i) load_cols(a.bias, wcol + 16 * i + 4 * fq, a.n, bias[i]);
   }
+  auto value = [&](int i, int j, float (&v)[4]) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      v[u] = (float)acc[i][j][u] * xs[j] * sc[i][u];
+      if constexpr (FUSED) v[u] = silu_f32(v[u]) * ((float)acc[i + 2][j][u] * xs[j] * sc[i + 2][u]);
+      else if (a.bias) v[u] += bias[i][u];
+    }
+  };
+  // Stored as they are, a wave's store would touch 16 rows with 32 bytes each: 16 tokens go through a patch of LDS and
+  // leave as whole row segments.  The slot of step S - 2 is free (everybody passed the last barrier after reading it).
+  uint8_t* patch = smem + (S & 1) * kSlotBytes + wave * 8192;
+  if (a.out_dtype == BGMOE_DT_FP32) store_tiles<Fp32, kTiles>(a, patch, row0 + m0 + 128 * wm, cnt - m0 - 128 * wm, wcol, value);
+  else if (a.out_dtype == BGMOE_DT_BF16) store_tiles<Bf16, kTiles>(a, patch, row0 + m0 + 128 * wm, cnt - m0 - 128 * wm, wcol, value);
+  else store_tiles<Fp16, kTiles>(a, patch, row0 + m0 + 128 * wm, cnt - m0 - 128 * wm, wcol, value);
 }
 
 // ---- row quantiser: one block per row, the row in registers between its maximum and its cast -----------------------------

@@ -34,3 +34,4 @@ template <int N>
 __device__ __forceinline__ void wait_vm() { emu::wait_vm(N); }
 __device__ __forceinline__ void block_barrier() { emu::block_barrier(); }
 __device__ __forceinline__ void lds_exchange_barrier() { emu::block_barrier(); }
+__device__ __forceinline__ void lds_reads_done() {}
