@@ -94,23 +94,34 @@ __device__ __forceinline__ void store8(void* row, int64_t c, int left, const flo
 
 // ---- one int8 scale per row: scale = max(amax, 1e-30) / 127, q = rint(v / scale), both IEEE fp32 ----------------------
 __device__ __forceinline__ float int8_scale(float amax) { return fmaxf(amax, 1e-30f) / 127.0f; }
-__device__ __forceinline__ uint32_t int8_of(float v, float scale) {
-  const float q = rintf(v / scale);
-  return (uint32_t)(int)(q == q ? fminf(fmaxf(q, -127.0f), 127.0f) : 0.0f) & 0xffu;
-}
+// Eight values of a row whose scale is `scale`.  While the scale is in (1e-30, 1e30) the quotient comes from one
+// reciprocal and a correction step (div_by_scale: the IEEE quotient at a third of its instructions); |v| <= 127 scale, so
+// nothing has to be clamped.  Else (rows of tiny or huge values, non-finite rows) by the division, NaN becoming 0.
 __device__ __forceinline__ void int8_store8(int8_t* p, int left, const float (&v)[8], float scale) {
   typedef unsigned int u32x2 __attribute__((ext_vector_type(2), aligned(1)));
+  int q[8];
+  if (scale_div_ok(scale)) {
+    const float r = 1.0f / scale;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = (int)rintf(div_by_scale(v[i], scale, r));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = rintf(v[i] / scale);
+      q[i] = f == f ? (int)fminf(fmaxf(f, -127.0f), 127.0f) : 0;
+    }
+  }
   if (left >= 8) {
     u32x2 o;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
-      o[j] = int8_of(v[4 * j], scale) | (int8_of(v[4 * j + 1], scale) << 8) | (int8_of(v[4 * j + 2], scale) << 16) |
-             (int8_of(v[4 * j + 3], scale) << 24);
+      o[j] = ((uint32_t)q[4 * j] & 0xffu) | (((uint32_t)q[4 * j + 1] & 0xffu) << 8) | (((uint32_t)q[4 * j + 2] & 0xffu) << 16) |
+             ((uint32_t)q[4 * j + 3] << 24);
     *reinterpret_cast<u32x2*>(p) = o;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < left) p[i] = (int8_t)int8_of(v[i], scale);
+      if (i < left) p[i] = (int8_t)q[i];
   }
 }
 

@@ -183,8 +183,8 @@ __global__ __launch_bounds__(1024) void gated_norm_kernel(NormArgs a) {
 }
 
 // `rows` is walked by gridDim.x blocks.  KIND order of the planes: post, pre, gate.
-template <typename T, int V>
-__global__ __launch_bounds__(1024) void gated_norm_backward_kernel(NormArgs a) {
+template <typename T, int V, int NT>
+__global__ __launch_bounds__(NT) void gated_norm_backward_kernel(NormArgs a) {
   __shared__ float s_sum[2][16][3];
   const int step = blockDim.x * 8;
   const float inv_h = 1.0f / (float)a.h;
@@ -306,9 +306,10 @@ __global__ __launch_bounds__(1024) void plane_sum_kernel(SumArgs a) {
   else store_one<T>(reinterpret_cast<uint8_t*>(a.out[kind]) + c * T::kBytes, s);
 }
 
+extern "C" { __attribute__((visibility("default"))) int bgmoe_n_force = 2; __attribute__((visibility("default"))) int bgmoe_nb_force = 1024; }
 // threads per row and vectors per thread: one vector up to 8192 columns, two above
 int threads_for(int h, int* vecs) {
-  *vecs = h > 8192 ? 2 : 1;
+  *vecs = h > 8192 ? 2 : bgmoe_n_force;
   return ((h + 8 * *vecs - 1) / (8 * *vecs) + BGMOE_WAVE - 1) / BGMOE_WAVE * BGMOE_WAVE;
 }
 // blocks of the gradient pass: enough to fill the chip (2048 threads per CU), each walking many rows
@@ -316,7 +317,7 @@ int64_t backward_blocks(int64_t rows, int h) {
   int vecs;
   const int threads = threads_for(h, &vecs);
   int64_t blocks = 256 * (2048 / threads);
-  if (blocks > 1024) blocks = 1024;
+  if (blocks > bgmoe_nb_force) blocks = bgmoe_nb_force;
   return rows < blocks ? rows : blocks;
 }
 
@@ -326,6 +327,7 @@ int run_forward(const NormArgs& a, hipStream_t st) {
   const int threads = threads_for(a.h, &vecs);
   BgmoeProf prof(BGMOE_K_GATED_NORM, st);
   if (vecs == 1) hipLaunchKernelGGL((gated_norm_kernel<T, 1>), bgmoe_grid(a.rows), dim3(threads), 0, st, a);
+  else if (vecs == 4) hipLaunchKernelGGL((gated_norm_kernel<T, 4>), bgmoe_grid(a.rows), dim3(threads), 0, st, a);
   else hipLaunchKernelGGL((gated_norm_kernel<T, 2>), bgmoe_grid(a.rows), dim3(threads), 0, st, a);
   return bgmoe_check_launch("gated_residual_norm");
 }
@@ -334,8 +336,9 @@ int run_backward(const NormArgs& a, const SumArgs& s, hipStream_t st) {
   int vecs;
   const int threads = threads_for(a.h, &vecs);
   BgmoeProf prof(BGMOE_K_GATED_NORM, st);
-  if (vecs == 1) hipLaunchKernelGGL((gated_norm_backward_kernel<T, 1>), dim3((unsigned)s.blocks), dim3(threads), 0, st, a);
-  else hipLaunchKernelGGL((gated_norm_backward_kernel<T, 2>), dim3((unsigned)s.blocks), dim3(threads), 0, st, a);
+  if (vecs == 1) hipLaunchKernelGGL((gated_norm_backward_kernel<T, 1, 1024>), dim3((unsigned)s.blocks), dim3(threads), 0, st, a);
+  else if (threads <= 512) hipLaunchKernelGGL((gated_norm_backward_kernel<T, 2, 512>), dim3((unsigned)s.blocks), dim3(threads), 0, st, a);
+  else hipLaunchKernelGGL((gated_norm_backward_kernel<T, 2, 1024>), dim3((unsigned)s.blocks), dim3(threads), 0, st, a);
   if (s.kinds) {
     const int64_t cols = (int64_t)s.kinds * s.h;
     hipLaunchKernelGGL((plane_sum_kernel<T>), dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, st, s);

@@ -6,8 +6,9 @@
 // columns of one token.  The accumulators are exact 32-bit integers (|sum| <= k * 128^2 < 2^31 for k <= 131071), so
 // no result depends on how K is cut; the scales enter once, in fp32, in the epilogue.
 //
-// Streaming kernel: a block owns 64 weight rows (4 waves x 16) and all of K, and walks the group's tokens in chunks of
-// 16, 32 or 64.  Weights and tokens go global -> LDS asynchronously in stages of 256 bytes of K (one 1 KB wave load
+// Streaming kernel, for groups of up to 32 rows: a block owns 64 weight rows (4 waves x 16), 16 or 32 tokens and all of K.
+// It is bound by the weights' stream from HBM (32 experts x 8 rows, gate + up of 2048 x 7168: 940 MB in 159 us, 5.9 TB/s).
+// Weights and tokens go global -> LDS asynchronously in stages of 256 bytes of K (one 1 KB wave load
 // covers 4 rows x 256 contiguous bytes) into a ring; a stage's 16-byte chunks are stored at position
 // chunk ^ (row & 15), so that the 16 lanes that read one chunk of 16 rows hit 16 different 16-byte slots of the 256
 // bytes the LDS serves at once.
@@ -75,9 +76,9 @@ __device__ __forceinline__ void group_rows(const Int8Args& a, int g, int64_t* ro
 
 template <bool FUSED, int MT>
 __device__ __forceinline__ void stream_chunk(const Int8Args& a, uint8_t* smem, const int8_t* wbase, int wrow0, int wrows,
-                                             const float* ws, const float* ws_up, int64_t row0, int t0, int cnt, int n0) {
+                                             const float* ws, const float* ws_up, int64_t row0, int cnt, int n0) {
   constexpr int kStage = (4 + MT) * kTile;             // 64 weight rows, 16 MT tokens
-  constexpr int kStages = kRingBytes / kStage;         // 4, 3, 2
+  constexpr int kStages = kRingBytes / kStage;         // 4 or 3
   constexpr int kLoads = 4 + MT;                       // wave loads per stage and wave
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -98,10 +99,10 @@ __device__ __forceinline__ void stream_chunk(const Int8Args& a, uint8_t* smem, c
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int row = 4 * (wave * MT + i) + lr;           // token of the chunk
-    x_off[i] = (uint32_t)min(row, cnt - 1 - t0) * (uint32_t)a.ldx + (uint32_t)((lc ^ (row & 15)) * 16);
+    x_off[i] = (uint32_t)min(row, cnt - 1) * (uint32_t)a.ldx + (uint32_t)((lc ^ (row & 15)) * 16);
   }
   const uint8_t* wsrc = uniform_ptr(reinterpret_cast<const uint8_t*>(wbase) + (int64_t)wrow0 * a.k);
-  const uint8_t* xsrc = uniform_ptr(reinterpret_cast<const uint8_t*>(a.x) + (row0 + t0) * a.ldx);
+  const uint8_t* xsrc = uniform_ptr(reinterpret_cast<const uint8_t*>(a.x) + row0 * a.ldx);
 
   auto issue = [&](int s) {
     const uint32_t d = lds0 + (uint32_t)(s % kStages) * kStage;
@@ -160,7 +161,7 @@ __device__ __forceinline__ void stream_chunk(const Int8Args& a, uint8_t* smem, c
     for (int i = 0; i < 4; ++i) sc[i] = (wave < 2 ? ws : ws_up)[min(col + i, a.n - 1)];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const float xs = a.xs[row0 + min(t0 + 16 * t + r, cnt - 1)];
+      const float xs = a.xs[row0 + min(16 * t + r, cnt - 1)];
       float v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = (float)acc[t][i] * xs * sc[i];
@@ -179,11 +180,10 @@ __device__ __forceinline__ void stream_chunk(const Int8Args& a, uint8_t* smem, c
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           v[i] = silu_f32(__int_as_float(acc[t][i])) * up[((wave * MT + t) * 4 + i) * 64 + lane];
-        const int tok = t0 + 16 * t + r;
+        const int tok = 16 * t + r;
         if (tok < cnt) store4(a, row0 + tok, col, v);
       }
     }
-    __syncthreads();
   } else {
     const int col = n0 + wave * 16 + 4 * q;
     float sc[4], bias[4];
@@ -194,7 +194,7 @@ __device__ __forceinline__ void stream_chunk(const Int8Args& a, uint8_t* smem, c
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const int tok = t0 + 16 * t + r;
+      const int tok = 16 * t + r;
       if (tok >= cnt) continue;
       const float xs = a.xs[row0 + tok];
       float v[4];
@@ -225,19 +225,8 @@ __global__ __launch_bounds__(256) void int8_stream_kernel(Int8Args a, int max_ro
   // this wave's 16 weight rows; a wave whose rows all lie past n repeats the last row and stores nothing
   const int wrow0 = min(n0 + (FUSED ? wave & 1 : wave) * 16, a.n - 1);
   const int wrows = min(16, a.n - wrow0);
-  for (int t0 = 0; t0 < cnt;) {
-    const int left = cnt - t0;
-    if (left <= 16) {
-      stream_chunk<FUSED, 1>(a, smem, wbase, wrow0, wrows, ws, ws_up, row0, t0, cnt, n0);
-      t0 += 16;
-    } else if (left <= 32) {
-      stream_chunk<FUSED, 2>(a, smem, wbase, wrow0, wrows, ws, ws_up, row0, t0, cnt, n0);
-      t0 += 32;
-    } else {
-      stream_chunk<FUSED, 4>(a, smem, wbase, wrow0, wrows, ws, ws_up, row0, t0, cnt, n0);
-      t0 += 64;
-    }
-  }
+  if (cnt <= 16) stream_chunk<FUSED, 1>(a, smem, wbase, wrow0, wrows, ws, ws_up, row0, cnt, n0);
+  else stream_chunk<FUSED, 2>(a, smem, wbase, wrow0, wrows, ws, ws_up, row0, cnt, n0);
 }
 
 // ---- tiled kernel: many rows per group ---------------------------------------------------------------------------------
@@ -257,8 +246,20 @@ __global__ __launch_bounds__(256) void int8_stream_kernel(Int8Args a, int max_ro
 // 16 different 16-byte slots of 256 bytes (no bank conflicts by the counter).
 // Bound: the chip's power.  With every CU at work the MFMAs alone run at 3.2 (32x32x32) and 3.6 (16x16x64) PFLOP/s on
 // normally distributed bytes, because the clock falls to about 1.6 GHz; this loop runs at 2.7.
-constexpr int kTM = 256, kTW = 256, kTK = 128, kSlots = 2;
-constexpr int kSlotBytes = (kTM + kTW) * kTK;
+// Tile<4, 8> is that macro tile.  Tile<2, 4> is 128 x 128 with 4 waves of 4 x 4 tiles and two 32 KB slots, two blocks per
+// CU: half the products per byte requested, four times the tiles, for problems whose large tiles would not fill the
+// chip (four slots, i.e. one block per CU with three steps in flight, are no faster with few tiles and slower with many).
+template <int WN_, int XT_> struct Tile {
+  static constexpr int WN = WN_, XT = XT_;              // waves along the weights; token tiles per wave
+  static constexpr int W = 64 * WN_, M = 32 * XT_;      // weight rows and tokens of a macro tile
+  static constexpr int kThreads = 128 * WN_;            // WN x 2 waves, each of which loads 32 rows of either operand
+  static constexpr int kSlot = (W + M) * 128;
+  static constexpr int kRing = 2 * kSlot;
+  static_assert(W == 64 * WN_ && M == 64 * WN_, "every wave loads 32 token rows and 32 weight rows");
+};
+typedef Tile<4, 8> Large;
+typedef Tile<2, 4> Small;
+constexpr int kTK = 128;
 constexpr int kMaxGroups = 1024;
 constexpr int kPanel = 8;                     // m-tiles that share their weight tiles in an XCD's L2
 
@@ -273,15 +274,15 @@ __device__ __forceinline__ void load_cols(const float* p, int col, int n, float 
     for (int i = 0; i < 4; ++i) v[i] = p[min(col + i, n - 1)];
   }
 }
-// Writes a wave's 128 tokens x 16 TILES columns: value(i, j, v) gives the lane's four columns of column tile i and token
+// Writes a wave's 16 XT tokens x 16 TILES columns: value(i, j, v) gives the lane's four columns of column tile i and token
 // tile j.  A row of the patch is one token's columns in 16-byte chunks at chunk ^ (row mod chunks per row).
-template <typename T, int TILES, typename V>
+template <typename T, int TILES, int XT, typename V>
 __device__ __forceinline__ void store_tiles(const Int8Args& a, uint8_t* patch, int64_t row0, int rows, int wcol, V value) {
   constexpr int kChunks = TILES * T::kBytes;           // 16-byte chunks per row
   constexpr int kPer = 16 / T::kBytes;                 // columns per chunk
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < XT; ++j) {
     if (16 * j >= rows) break;                         // wave-uniform
     uint8_t* buf = patch + (j & 1) * 4096;             // two patches: the next tile is written while this one leaves
 #pragma unroll
@@ -325,14 +326,15 @@ __device__ __forceinline__ void store_tiles(const Int8Args& a, uint8_t* patch, i
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
-template <bool FUSED>
-__global__ __launch_bounds__(512) void int8_tiled_kernel(Int8Args a, int groups, int min_rows) {
+template <bool FUSED, typename TL>
+__global__ __launch_bounds__(TL::kThreads) void int8_tiled_kernel(Int8Args a, int groups, int min_rows) {
+  constexpr int kTM = TL::M, kSlotBytes = TL::kSlot, XT = TL::XT, WN = TL::WN;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int s_tiles[kMaxGroups + 1];
-  constexpr int kCols = FUSED ? 128 : 256;
+  constexpr int kCols = FUSED ? TL::W / 2 : TL::W;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wn = wave & 3, wm = wave >> 2;
+  const int wn = wave % WN, wm = wave / WN;
   const int ntn = (a.n + kCols - 1) / kCols;
 
   // ---- which (group, m-tile, n-tile): block b runs on XCD b % 8 and takes items of that eighth of the list ----
@@ -394,9 +396,9 @@ __global__ __launch_bounds__(512) void int8_tiled_kernel(Int8Args a, int groups,
   const int lr = lane >> 3;
   const int lc[2] = {(lane & 7) ^ (lane >> 4), (lane & 7) ^ (4 + (lane >> 4))};      // source chunk in even and odd loads
   const uint8_t* xsrc = uniform_ptr(reinterpret_cast<const uint8_t*>(a.x) + (row0 + m0) * a.ldx);
-  const bool up = FUSED && wave >= 4;
+  const bool up = FUSED && wave >= WN;
   const int8_t* wmat = up ? a.w1 + grp * a.w1_group : a.w0 + grp * a.w0_group;
-  const int first_row = min(n0 + (FUSED ? 32 * (wave & 3) : 32 * wave), a.n - 1);
+  const int first_row = min(n0 + 32 * (FUSED ? wave % WN : wave), a.n - 1);
   const uint8_t* wsrc = uniform_ptr(reinterpret_cast<const uint8_t*>(wmat) + (int64_t)first_row * a.k);
   uint32_t x_off[4], w_off[4];
 #pragma unroll
@@ -436,26 +438,28 @@ __global__ __launch_bounds__(512) void int8_tiled_kernel(Int8Args a, int groups,
   for (int h = 0; h < 2; ++h) f_off[h] = fr * kTK + (((4 * h + fq) ^ ((fr >> 1) & 7)) * 16);
   int a_off[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) a_off[i] = kTM * kTK + 16 * kTK * (FUSED ? 8 * (i >> 1) + 2 * wn + (i & 1) : 4 * wn + i);
-  const int b_off = 128 * kTK * wm;
+  for (int i = 0; i < 4; ++i) a_off[i] = kTM * kTK + 16 * kTK * (FUSED ? 2 * WN * (i >> 1) + 2 * wn + (i & 1) : 4 * wn + i);
+  const int b_off = kTM / 2 * kTK * wm;
   // the weights of a half are double-buffered; a token tile's register is refilled as soon as it has been multiplied
-  intx4 w0[4], w1[4], x[8];
+  intx4 w0[4], w1[4], x[XT];
   auto read_w = [&](int s, int h, int i) {
     return *reinterpret_cast<const intx4*>(smem + (s & 1) * kSlotBytes + f_off[h] + a_off[i]);
   };
   auto read_x = [&](int s, int h, int j) {
     return *reinterpret_cast<const intx4*>(smem + (s & 1) * kSlotBytes + f_off[h] + b_off + 16 * kTK * j);
   };
-  intx4 acc[4][8];
+  intx4 acc[4][XT];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = intx4{0, 0, 0, 0};
-  // multiplies w with x while reading half rh of step rs into wn and x; LOAD: requests step ls
+    for (int j = 0; j < XT; ++j) acc[i][j] = intx4{0, 0, 0, 0};
+  // multiplies w with x while reading half rh of step rs into wnext and x; load: requests step ls
   auto half = [&](auto load, const intx4 (&w)[4], intx4 (&wnext)[4], int rs, int rh, int ls) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (decltype(load)::value) issue_one(ls, j);
+    for (int j = 0; j < XT; ++j) {
+      if constexpr (decltype(load)::value)
+#pragma unroll
+        for (int u = 0; u < 8 / XT; ++u) issue_one(ls, j * (8 / XT) + u);
       if (j < 4) wnext[j] = read_w(rs, rh, j);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -470,7 +474,7 @@ __global__ __launch_bounds__(512) void int8_tiled_kernel(Int8Args a, int groups,
   wait_vm<8>();
   block_barrier();
   // a wave without a row of either operand inside the problem only loads and keeps the barriers
-  const bool live = m0 + 128 * wm < cnt && n0 + (FUSED ? 32 : 64) * wn < a.n;
+  const bool live = m0 + kTM / 2 * wm < cnt && n0 + (FUSED ? 32 : 64) * wn < a.n;
   if (!live) {
     for (int s = 0; s + 1 < S; ++s) {
       wait_vm<0>();
@@ -482,7 +486,7 @@ __global__ __launch_bounds__(512) void int8_tiled_kernel(Int8Args a, int groups,
 #pragma unroll
   for (int i = 0; i < 4; ++i) w0[i] = read_w(0, 0, i);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = read_x(0, 0, j);
+  for (int j = 0; j < XT; ++j) x[j] = read_x(0, 0, j);
   auto next_step = [&] {                      // step s + 1 is there; everybody has read step s
     wait_vm<0>();
     lds_reads_done();
@@ -503,7 +507,7 @@ __global__ __launch_bounds__(512) void int8_tiled_kernel(Int8Args a, int groups,
   half(No{}, w1, w0, S - 1, 0, 0);
   half(No{}, w0, w1, S - 1, 1, 0);
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int j = 0; j < XT; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w1[i], x[j], acc[i][j], 0, 0, 0);
 
@@ -512,9 +516,10 @@ __global__ __launch_bounds__(512) void int8_tiled_kernel(Int8Args a, int groups,
   const float* ws0 = a.ws0 + grp * a.ws0_group;
   const float* ws1 = FUSED ? a.ws1 + grp * a.ws1_group : nullptr;
   const int wcol = n0 + 16 * kTiles * wn;     // this wave's first column
-  float sc[4][4], bias[kTiles][4], xs[8];
+  const int wrow = m0 + kTM / 2 * wm;         // and first token
+  float sc[4][4], bias[kTiles][4], xs[XT];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) xs[j] = a.xs[row0 + min(m0 + 128 * wm + 16 * j + fr, cnt - 1)];
+  for (int j = 0; j < XT; ++j) xs[j] = a.xs[row0 + min(wrow + 16 * j + fr, cnt - 1)];
 #pragma unroll
   for (int i = 0; i < 4; ++i) load_cols(i < kTiles ? ws0 : ws1, wcol + 16 * (i % kTiles) + 4 * fq, a.n, sc[i]);
   if (a.bias) {
@@ -532,9 +537,107 @@ __global__ __launch_bounds__(512) void int8_tiled_kernel(Int8Args a, int groups,
   // Stored as they are, a wave's store would touch 16 rows with 32 bytes each: 16 tokens go through a patch of LDS and
   // leave as whole row segments.  The slot of step S - 2 is free (everybody passed the last barrier after reading it).
   uint8_t* patch = smem + (S & 1) * kSlotBytes + wave * 8192;
-  if (a.out_dtype == BGMOE_DT_FP32) store_tiles<Fp32, kTiles>(a, patch, row0 + m0 + 128 * wm, cnt - m0 - 128 * wm, wcol, value);
-  else if (a.out_dtype == BGMOE_DT_BF16) store_tiles<Bf16, kTiles>(a, patch, row0 + m0 + 128 * wm, cnt - m0 - 128 * wm, wcol, value);
-  else store_tiles<Fp16, kTiles>(a, patch, row0 + m0 + 128 * wm, cnt - m0 - 128 * wm, wcol, value);
+  if (a.out_dtype == BGMOE_DT_FP32) store_tiles<Fp32, kTiles, XT>(a, patch, row0 + wrow, cnt - wrow, wcol, value);
+  else if (a.out_dtype == BGMOE_DT_BF16) store_tiles<Bf16, kTiles, XT>(a, patch, row0 + wrow, cnt - wrow, wcol, value);
+  else store_tiles<Fp16, kTiles, XT>(a, patch, row0 + wrow, cnt - wrow, wcol, value);
+}
+
+// ---- split kernel: one weight matrix and few rows, the dense decode case ------------------------------------------------
+// There are too few (row block, token block) pairs to fill the chip when each walks all of K, so the eight waves of a
+// block take an eighth of K each for the same 16 RT weight rows and 16 MT tokens and add their integer sums through
+// LDS at the end: no workspace, no second launch.  Operands go straight from global memory to the MFMA registers: lane
+// (r, q) reads 32 contiguous bytes of row r per 128-byte step (K is permuted alike for both operands: the first 16
+// bytes feed one MFMA, the second 16 the next), so that four lanes cover a line.
+template <int RT, int MT>
+__global__ __launch_bounds__(512) void int8_split_kernel(Int8Args a) {
+  constexpr int kWaves = 8;
+  __shared__ __align__(16) int s_sum[kWaves][MT * RT > 4 ? 4 : MT * RT][256];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int n0 = blockIdx.x * 16 * RT;
+  const int64_t t0 = (int64_t)blockIdx.y * 16 * MT;
+  const int chunks = a.k >> 4, S = (a.k + 127) / 128, whole = a.k / 128;
+  const int s0 = S * wave / kWaves, s1 = S * (wave + 1) / kWaves;
+  const uint8_t* wp[RT];
+  const uint8_t* xp[MT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+    wp[i] = reinterpret_cast<const uint8_t*>(a.w0) + (int64_t)min(n0 + 16 * i + r, a.n - 1) * a.k + 32 * q;
+#pragma unroll
+  for (int j = 0; j < MT; ++j)
+    xp[j] = reinterpret_cast<const uint8_t*>(a.x) + min(t0 + 16 * j + r, a.m - 1) * a.ldx + 32 * q;
+  intx4 acc[RT][MT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = intx4{0, 0, 0, 0};
+  auto step = [&](const intx4 (&w)[RT][2], const intx4 (&x)[MT][2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i][h], x[j][h], acc[i][j], 0, 0, 0);
+  };
+  constexpr int kUnroll = RT * MT >= 8 ? 2 : 4;
+  int s = s0;
+  for (; s + kUnroll <= min(s1, whole); s += kUnroll) {
+    intx4 w[kUnroll][RT][2], x[kUnroll][MT][2];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i) w[u][i][h] = gload_x4(wp[i] + (s + u) * 128 + 16 * h);
+#pragma unroll
+        for (int j = 0; j < MT; ++j) x[u][j][h] = gload_x4(xp[j] + (s + u) * 128 + 16 * h);
+      }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) step(w[u], x[u]);
+  }
+  for (; s < s1; ++s) {
+    intx4 w[RT][2], x[MT][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool in = 8 * s + 2 * q + h < chunks;
+#pragma unroll
+      for (int i = 0; i < RT; ++i) w[i][h] = in ? gload_x4(wp[i] + s * 128 + 16 * h) : intx4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < MT; ++j) x[j][h] = in ? gload_x4(xp[j] + s * 128 + 16 * h) : intx4{0, 0, 0, 0};
+    }
+    step(w, x);
+  }
+
+  // sums over the waves, up to four 16 x 16 tiles at a time; a thread then holds four columns of one token
+  constexpr int kAll = RT * MT, kAtOnce = kAll > 4 ? 4 : kAll;
+#pragma unroll
+  for (int base = 0; base < kAll; base += kAtOnce) {
+    if (base) __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+      *reinterpret_cast<intx4*>(&s_sum[wave][u][lane * 4]) = acc[(base + u) / MT][(base + u) % MT];
+    __syncthreads();
+    const int u = threadIdx.x >> 6;
+    if (u < kAtOnce) {
+      intx4 sum = *reinterpret_cast<const intx4*>(&s_sum[0][u][lane * 4]);
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) sum += *reinterpret_cast<const intx4*>(&s_sum[w][u][lane * 4]);
+      const int col = n0 + 16 * ((base + u) / MT) + 4 * q;
+      const int64_t tok = t0 + 16 * ((base + u) % MT) + r;
+      if (tok < a.m && col < a.n) {
+        float sc[4], bias[4] = {0.0f, 0.0f, 0.0f, 0.0f}, v[4];
+        load_cols(a.ws0, col, a.n, sc);
+        if (a.bias) load_cols(a.bias, col, a.n, bias);
+        const float xs = a.xs[tok];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = (float)sum[i] * xs * sc[i];
+          if (a.bias) v[i] += bias[i];
+        }
+        store4(a, tok, col, v);
+      }
+    }
+  }
 }
 
 // ---- row quantiser: one block per row, the row in registers between its maximum and its cast -----------------------------
@@ -599,13 +702,13 @@ __global__ __launch_bounds__(1024) void int8_quant_kernel(const uint8_t* __restr
 
 template <typename T>
 int run_quant(const void* x, int64_t stride, int64_t rows, int k, int8_t* q, float* scale, hipStream_t st) {
-  const int vecs = k <= 8192 ? 1 : (k <= 16384 ? 2 : 0);
-  int threads = 1024;
-  if (vecs) threads = ((k + 8 * vecs - 1) / (8 * vecs) + BGMOE_WAVE - 1) / BGMOE_WAVE * BGMOE_WAVE;
+  // two vectors per thread: 8192 x 7168 bf16 in 31.5 us (5.6 TB/s), 1 x 7168 in 3.2 us; one vector (896 threads a row)
+  // 68 and 4.0 us, four 31.1 and 3.8 us, eight 34.6 and 5.2 us
+  const bool held = k <= 16384;
+  const int threads = held ? ((k + 15) / 16 + BGMOE_WAVE - 1) / BGMOE_WAVE * BGMOE_WAVE : 1024;
   const dim3 grid = bgmoe_grid(rows), block(threads);
   BgmoeProf prof(BGMOE_K_INT8_QUANT, st);
-  if (vecs == 1) hipLaunchKernelGGL((int8_quant_kernel<T, 1>), grid, block, 0, st, (const uint8_t*)x, stride, rows, k, q, scale);
-  else if (vecs == 2) hipLaunchKernelGGL((int8_quant_kernel<T, 2>), grid, block, 0, st, (const uint8_t*)x, stride, rows, k, q, scale);
+  if (held) hipLaunchKernelGGL((int8_quant_kernel<T, 2>), grid, block, 0, st, (const uint8_t*)x, stride, rows, k, q, scale);
   else hipLaunchKernelGGL((int8_quant_kernel<T, 0>), grid, block, 0, st, (const uint8_t*)x, stride, rows, k, q, scale);
   return bgmoe_check_launch("int8_quant_rows");
 }
@@ -617,40 +720,110 @@ int check_sizes(const char* what, int64_t m, int n, int k, int out_dtype) {
   return BGMOE_OK;
 }
 
-// Groups of up to kStreamRows rows are streamed, larger ones tiled; each kernel skips the other's groups.
-constexpr int kStreamRows = 64;
+// Grouped: groups of up to kStreamRows rows are streamed, larger ones tiled; each kernel skips the other's groups.  Equal
+// groups, 32 experts x (gate + up of 2048) x 7168 and 64 experts x 7168 x 2048, streamed | tiled 128 x 128:
+// 32 rows 167 | 168, 203 | 197 us; 40 rows 180 | 174, 212 | 200 us; 64 rows 194 | 178, 233 | 217 us.
+constexpr int kStreamRows = 32;
+// The tile of the larger groups goes by the average, which is what the host knows.  128 x 128 | 256 x 256:
+// 96 rows 195 | 214 us, 128 rows 206 | 220, 192 rows 292 | 250, 512 rows 594 | 458 (32 experts); 128 rows 243 | 267,
+// 256 rows 385 | 309 us (64 experts).
+constexpr int kSmallTileRows = 160;
+
+template <bool FUSED, typename TL>
+int run_tiled(const char* what, const Int8Args& a, int groups, hipStream_t st) {
+  // a bound on the m-tiles of groups above the streaming limit, whatever the counts
+  const int64_t m_tiles = a.seqlens ? a.m / TL::M + min((int64_t)groups, a.m / (kStreamRows + 1)) : (a.m + TL::M - 1) / TL::M;
+  constexpr int kCols = FUSED ? TL::W / 2 : TL::W;
+  const int64_t blocks = (m_tiles * ((a.n + kCols - 1) / kCols) + 7) / 8 * 8;
+  BGMOE_REQUIRE(blocks <= 1 << 22, "%s: m=%lld x n=%d is too large for one launch", what, (long long)a.m, a.n);
+  hipLaunchKernelGGL((int8_tiled_kernel<FUSED, TL>), dim3((unsigned)blocks), dim3(TL::kThreads), TL::kRing, st, a, groups,
+                     kStreamRows);
+  return bgmoe_check_launch(what);
+}
+
+template <bool FUSED>
+int run_stream(const char* what, const Int8Args& a, int groups, hipStream_t st) {
+  constexpr int kCols = FUSED ? 32 : 64;
+  const dim3 grid((unsigned)((a.n + (int64_t)kCols - 1) / kCols), (unsigned)groups);
+  hipLaunchKernelGGL(int8_stream_kernel<FUSED>, grid, dim3(256), kRingBytes, st, a, kStreamRows);
+  return bgmoe_check_launch(what);
+}
+
+template <bool FUSED>
+int run_grouped(const char* what, const Int8Args& a, int groups, hipStream_t st) {
+  const int rc = run_stream<FUSED>(what, a, groups, st);
+  if (rc != BGMOE_OK || a.m <= kStreamRows) return rc;
+  return a.m <= (int64_t)kSmallTileRows * groups ? run_tiled<FUSED, Small>(what, a, groups, st)
+                                                 : run_tiled<FUSED, Large>(what, a, groups, st);
+}
+
+template <int RT, int MT>
+int run_split(const char* what, const Int8Args& a, hipStream_t st) {
+  const dim3 grid((unsigned)((a.n + (int64_t)16 * RT - 1) / (16 * RT)), (unsigned)((a.m + 16 * MT - 1) / (16 * MT)));
+  hipLaunchKernelGGL((int8_split_kernel<RT, MT>), grid, dim3(512), 0, st, a);
+  return bgmoe_check_launch(what);
+}
+
+// Dense: the form with the smallest estimated time.  The estimates (microseconds) are fits to graph-timed runs over
+// n x k = 4096 x 7168, 7168 x 2048, 1024 x 1024, 512 x 512 and 36864 x 7168, m = 1 .. 4096:
+//   split RT x MT   a launch, a tile's share of the reduction, and the bytes its blocks request at 37 GB/s per CU
+//   stream          a stage costs 0.33 (16 tokens) or 0.66 (32) while two blocks share a CU; the weights at 5.9 TB/s
+//   tiled 128       0.63 per step until about 300 tiles are at work, then 0.0021 per tile
+//   tiled 256       1.15 per step, 1.65 when every CU has a tile
+// Measured against one another at 4096 x 7168: m = 1 split 6.5, stream 11.9; m = 64 split 15.2, tiled 128 38; m = 256
+// split 30.0, tiled 128 39.9; m = 512 split 57, tiled 128 40.5, tiled 256 67.8; m = 2048 tiled 128 66.0, tiled 256 72.0;
+// m = 4096 tiled 128 126, tiled 256 94 us.  At 36864 x 7168, m = 16: stream 44.2, split 52.3 us.
+int run_dense(const char* what, const Int8Args& a, hipStream_t st) {
+  const double n = a.n, k = a.k, m = (double)a.m, steps = (a.k + kTK - 1) / kTK;
+  auto ceil_div = [](int64_t x, int64_t y) { return (double)((x + y - 1) / y); };
+  auto split = [&](int rt, int mt) {
+    const double blocks = ceil_div(a.n, 16 * rt) * ceil_div(a.m, 16 * mt), rounds = blocks > 256 ? blocks / 256 : 1;
+    const double rows = 16 * rt + (m < 16 * mt ? m : 16 * mt), asked = rounds * rows * k / 37e3, hbm = n * k / 4.9e6;
+    return 2.6 + 0.11 * rt * mt + (asked > hbm ? asked : hbm);
+  };
+  const double tiles_s = ceil_div(a.n, 128) * ceil_div(a.m, 128), tiles_l = ceil_div(a.n, 256) * ceil_div(a.m, 256);
+  const double stage = 0.33 * ceil_div(a.m, 16) * ceil_div(a.k, kStageK) * ceil_div((int64_t)ceil_div(a.n, 64), 512);
+  const double weights = n * k / 5.9e6;
+  double best = 6.0 + steps * (tiles_l > 128 ? 1.65 : 1.15) * ceil_div((int64_t)tiles_l, 256);
+  int form = 0;
+  auto consider = [&](int which, double t) {
+    if (t < best) best = t, form = which;
+  };
+  consider(1, 4.3 + steps * (tiles_s < 300 ? 0.63 : 0.0021 * tiles_s));
+  if (a.m <= kStreamRows) consider(2, 3.0 + (stage > weights ? stage : weights));
+  if (a.m <= 65535 * 16) {
+    consider(11, split(1, 1));
+    consider(22, split(2, 2));
+    consider(24, split(2, 4));
+    consider(44, split(4, 4));
+  }
+  switch (form) {
+    case 11: return run_split<1, 1>(what, a, st);
+    case 22: return run_split<2, 2>(what, a, st);
+    case 24: return run_split<2, 4>(what, a, st);
+    case 44: return run_split<4, 4>(what, a, st);
+    case 2: return run_stream<false>(what, a, 1, st);
+    case 1: return run_tiled<false, Small>(what, a, 1, st);
+    default: return run_tiled<false, Large>(what, a, 1, st);
+  }
+}
 
 int run_gemm(const char* what, const Int8Args& a, int groups, hipStream_t st) {
-  const bool fused = a.w1 != nullptr;
-  const int cols = fused ? 32 : 64;
-  const int64_t tiles = ((int64_t)a.n + cols - 1) / cols;
-  BGMOE_REQUIRE(tiles <= 1 << 24, "%s: n=%d is too wide", what, a.n);
-  const bool grouped = a.seqlens != nullptr;
+  BGMOE_REQUIRE(a.n <= 1 << 22, "%s: n=%d is too wide", what, a.n);
   BgmoeProf prof(BGMOE_K_INT8_GEMM, st);
-  if (grouped || a.m <= kStreamRows) {
-    const dim3 grid((unsigned)tiles, (unsigned)groups), block(256);
-    if (fused) hipLaunchKernelGGL(int8_stream_kernel<true>, grid, block, kRingBytes, st, a, kStreamRows);
-    else hipLaunchKernelGGL(int8_stream_kernel<false>, grid, block, kRingBytes, st, a, kStreamRows);
-  }
-  if (a.m > kStreamRows) {                    // a bound on the m-tiles of groups above the limit, whatever the counts
-    const int64_t m_tiles = grouped ? a.m / kTM + min((int64_t)groups, a.m / (kStreamRows + 1)) : (a.m + kTM - 1) / kTM;
-    const int64_t items = m_tiles * ((a.n + (fused ? 127 : 255)) / (fused ? 128 : 256));
-    const int64_t blocks = (items + 7) / 8 * 8;
-    BGMOE_REQUIRE(blocks <= 1 << 22, "%s: m=%lld x n=%d is too large for one launch", what, (long long)a.m, a.n);
-    const dim3 grid((unsigned)blocks), block(512);
-    if (fused) hipLaunchKernelGGL(int8_tiled_kernel<true>, grid, block, kSlots * kSlotBytes, st, a, groups, kStreamRows);
-    else hipLaunchKernelGGL(int8_tiled_kernel<false>, grid, block, kSlots * kSlotBytes, st, a, groups, kStreamRows);
-  }
-  return bgmoe_check_launch(what);
+  if (a.seqlens == nullptr) return run_dense(what, a, st);
+  return a.w1 ? run_grouped<true>(what, a, groups, st) : run_grouped<false>(what, a, groups, st);
 }
 
 }  // namespace
 
 int bgmoe_internal_init_int8_gemm() {
-  const struct { const void* fn; int bytes; } fns[4] = {{(const void*)int8_stream_kernel<false>, kRingBytes},
-                                                        {(const void*)int8_stream_kernel<true>, kRingBytes},
-                                                        {(const void*)int8_tiled_kernel<false>, kSlots * kSlotBytes},
-                                                        {(const void*)int8_tiled_kernel<true>, kSlots * kSlotBytes}};
+  const struct { const void* fn; int bytes; } fns[] = {{(const void*)int8_stream_kernel<false>, kRingBytes},
+                                                       {(const void*)int8_stream_kernel<true>, kRingBytes},
+                                                       {(const void*)int8_tiled_kernel<false, Large>, Large::kRing},
+                                                       {(const void*)int8_tiled_kernel<true, Large>, Large::kRing},
+                                                       {(const void*)int8_tiled_kernel<false, Small>, Small::kRing},
+                                                       {(const void*)int8_tiled_kernel<true, Small>, Small::kRing}};
   for (const auto& f : fns) {
     const hipError_t err = hipFuncSetAttribute(f.fn, hipFuncAttributeMaxDynamicSharedMemorySize, f.bytes);
     if (err != hipSuccess) {

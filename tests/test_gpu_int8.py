@@ -80,7 +80,7 @@ def test_quantiser_edges(dev):
 # ---- dense -------------------------------------------------------------------------------------------------------------
 # m, n, k: one token, tile edges on every side, K tails inside a stage, many rows
 DENSE = [(1, 64, 256), (1, 33, 16), (2, 1, 48), (16, 64, 512), (17, 65, 272), (31, 100, 1024), (33, 129, 496), (64, 64, 1296),
-         (65, 31, 64), (130, 257, 304), (257, 300, 144), (300, 512, 256)]
+         (65, 31, 64), (130, 257, 304), (257, 300, 144), (300, 512, 256), (20, 8200, 64), (33, 8200, 80), (700, 1300, 528), (1100, 700, 400)]
 
 
 @pytest.mark.parametrize("shape", DENSE, ids=str)
