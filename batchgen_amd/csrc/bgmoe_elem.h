@@ -79,6 +79,28 @@ __device__ __forceinline__ void load8(const void* row, int64_t c, int left, floa
     for (int i = 0; i < 8; ++i) v[i] = i < left ? load_one<T>(p + i * T::kBytes) : 0.0f;
   }
 }
+// the same, still packed: half the registers for the two-byte types
+template <typename T> struct Packed8 { u32x4 v[T::kBytes / 2]; };
+template <typename T>
+__device__ __forceinline__ Packed8<T> load8_packed(const void* row, int64_t c, int left) {
+  const uint8_t* p = reinterpret_cast<const uint8_t*>(row) + c * T::kBytes;
+  Packed8<T> r;
+  if (left >= 8) {
+    r.v[0] = load16(p);
+    if constexpr (T::kBytes == 4) r.v[1] = load16(p + 16);
+  } else {
+    typename T::raw e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = i < left ? reinterpret_cast<const typename T::raw*>(p)[i] : (typename T::raw)0;
+    __builtin_memcpy(&r, e, sizeof(r));
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const Packed8<T>& r, float (&v)[8]) {
+  unpack16<T>(r.v[0], v);
+  if constexpr (T::kBytes == 4) unpack16<T>(r.v[1], v + 4);
+}
 template <typename T>
 __device__ __forceinline__ void store8(void* row, int64_t c, int left, const float (&v)[8]) {
   uint8_t* p = reinterpret_cast<uint8_t*>(row) + c * T::kBytes;

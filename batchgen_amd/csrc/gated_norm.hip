@@ -23,6 +23,7 @@
 namespace {
 
 constexpr int kMaxH = 16384;
+constexpr int kAccBytes = 3 * 8 * 4;          // LDS accumulators of a thread of the gradient pass
 
 struct NormArgs {
   const void *block, *residual, *post, *gate, *pre;
@@ -182,62 +183,104 @@ __global__ __launch_bounds__(1024) void gated_norm_kernel(NormArgs a) {
   }
 }
 
-// `rows` is walked by gridDim.x blocks.  KIND order of the planes: post, pre, gate.
-template <typename T, int V, int NT>
-__global__ __launch_bounds__(NT) void gated_norm_backward_kernel(NormArgs a) {
+// Rows are walked by gridDim.x blocks; the next row's operands are requested, still packed, before this row's exchange of
+// sums, so that a CU always has a row (57 KB at h = 7168) on its way while its VALU (about 45 operations per element)
+// works on another.  What the blocks sum over their rows lives in LDS, eight floats per thread and kind (in registers it
+// takes the place of that next row, or of a second block per CU).  Order of the planes: post, pre, gate.
+// ACC_LDS = false (rows wider than LDS holds, h > 8192): accumulators in registers.
+template <typename T, int V, bool ACC_LDS>
+__global__ __launch_bounds__(1024) void gated_norm_backward_kernel(NormArgs a) {
+  extern __shared__ __align__(16) float s_acc[];         // [kind][thread * 8 + i]
   __shared__ float s_sum[2][16][3];
   const int step = blockDim.x * 8;
   const float inv_h = 1.0f / (float)a.h;
-  float d1[V][8], d2[V][8], dg[V][8];
+  float racc[ACC_LDS ? 1 : 3][V][8];
+  auto add = [&](int kind, int u, const float (&v)[8]) {
+    if constexpr (ACC_LDS) {
+      float4* p = reinterpret_cast<float4*>(s_acc + kind * step + threadIdx.x * 8);
 #pragma unroll
-  for (int u = 0; u < V; ++u)
+      for (int q = 0; q < 2; ++q) {
+        float4 o = p[q];
+        o.x += v[4 * q]; o.y += v[4 * q + 1]; o.z += v[4 * q + 2]; o.w += v[4 * q + 3];
+        p[q] = o;
+      }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) d1[u][i] = d2[u][i] = dg[u][i] = 0.0f;
+      for (int i = 0; i < 8; ++i) racc[kind][u][i] += v[i];
+    }
+  };
+#pragma unroll
+  for (int kind = 0; kind < 3; ++kind) {
+    if constexpr (ACC_LDS) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s_acc[kind * step + threadIdx.x * 8 + i] = 0.0f;
+    } else {
+#pragma unroll
+      for (int u = 0; u < V; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) racc[kind][u][i] = 0.0f;
+    }
+  }
+  const bool norm = a.pre != nullptr && a.dn != nullptr;
+  struct Row { Packed8<T> b[V], r[V], dy[V], dn[V]; };
+  auto request = [&](int64_t row) {
+    Row o;
+    const int64_t base = row * a.h;
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      const int c = threadIdx.x * 8 + u * step, left = a.h - c;
+      o.b[u] = load8_packed<T>(a.block, base + c, left);
+      o.r[u] = load8_packed<T>(a.residual, base + c, left);
+      o.dy[u] = a.dy ? load8_packed<T>(a.dy, base + c, left) : Packed8<T>{};
+      o.dn[u] = norm ? load8_packed<T>(a.dn, base + c, left) : Packed8<T>{};
+    }
+    return o;
+  };
+  constexpr bool kAhead = ACC_LDS && T::kBytes == 2;     // (fp32 rows have twice the bytes in flight without it)
+  Row next;
+  if (kAhead) next = request(blockIdx.x);
   int slot = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, slot ^= 1) {
     const int64_t base = row * a.h;
+    if (!kAhead) next = request(row);
     const float token = a.gate_mode == BGMOE_GATE_TOKEN ? load_param1<T>(a.gate, (a.param_fp32 & 2) != 0, row) : 1.0f;
     const float i1 = a.post ? a.i_post[row] : 1.0f;
-    const float i2 = a.pre ? a.i_pre[row] : 0.0f;
-    // bh: b * i1;  c1: w1 (1 without a norm behind the block);  yh: y * i2;  e: dy + i2 * t
+    const float i2 = norm ? a.i_pre[row] : 0.0f;         // without a gradient through that norm y plays no part
+    // bh: b * i1;  w1 (1 without a norm behind the block);  yh: y * i2;  e: dy + i2 * t;  sg: s g without a token's gate
     float bh[V][8], yh[V][8], e[V][8], sg[V][8], w1[V][8];
     float sum[3] = {0.0f, 0.0f, 0.0f};                   // t yh, c' bh e, c' bh yh  (c' without the token's gate)
 #pragma unroll
     for (int u = 0; u < V; ++u) {
       const int c = threadIdx.x * 8 + u * step, left = a.h - c;
-      float dn[8], w2[8];
-      load8<T>(a.block, base + c, left, bh[u]);
-      load8<T>(a.residual, base + c, left, yh[u]);
-      if (a.dy) load8<T>(a.dy, base + c, left, e[u]);
-      else
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[u][i] = 0.0f;
+      float dn[8], w2[8], dw2[8];
       load_gate8<T>(a, row, c, left, 1.0f, sg[u]);
       if (a.post) load_param8<T>(a.post, (a.param_fp32 & 1) != 0, c, left, w1[u]);
       else
 #pragma unroll
         for (int i = 0; i < 8; ++i) w1[u][i] = 1.0f;
-      const bool norm = a.pre != nullptr && a.dn != nullptr;
-      if (norm) {
-        load8<T>(a.dn, base + c, left, dn);
-        load_param8<T>(a.pre, (a.param_fp32 & 4) != 0, c, left, w2);
-      }
+      if (norm) load_param8<T>(a.pre, (a.param_fp32 & 4) != 0, c, left, w2);
+      unpack8<T>(next.b[u], bh[u]);
+      unpack8<T>(next.r[u], yh[u]);
+      unpack8<T>(next.dy[u], e[u]);
+      unpack8<T>(next.dn[u], dn);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         bh[u][i] *= i1;
-        const float cg = sg[u][i] * w1[u][i];
         const float y = __builtin_fmaf(token * sg[u][i], bh[u][i] * w1[u][i], yh[u][i]);
-        yh[u][i] = norm && i < left ? y * i2 : 0.0f;      // without a gradient through that norm y plays no part
+        yh[u][i] = norm && i < left ? y * i2 : 0.0f;
         if (norm) {
           const float t = dn[i] * w2[i];
           sum[0] = __builtin_fmaf(t, yh[u][i], sum[0]);
           e[u][i] = __builtin_fmaf(i2, t, e[u][i]);
-          d2[u][i] = __builtin_fmaf(dn[i], yh[u][i], d2[u][i]);
+          dw2[i] = dn[i] * yh[u][i];
         }
-        sum[1] = __builtin_fmaf(cg * bh[u][i], e[u][i], sum[1]);
-        sum[2] = __builtin_fmaf(cg * bh[u][i], yh[u][i], sum[2]);
+        const float cb = sg[u][i] * w1[u][i] * bh[u][i];
+        sum[1] = __builtin_fmaf(cb, e[u][i], sum[1]);
+        sum[2] = __builtin_fmaf(cb, yh[u][i], sum[2]);
       }
+      if (norm && a.want_pre) add(1, u, dw2);
     }
+    if (kAhead && row + gridDim.x < a.rows) next = request(row + gridDim.x);
     block_sum<3>(sum, &s_sum[slot]);
     const float m = i2 * (sum[0] * inv_h);               // i2 * mean(t yh)
     const float cdb = sum[1] - m * sum[2];               // sum(c' Dy bh)
@@ -249,15 +292,13 @@ __global__ __launch_bounds__(NT) void gated_norm_backward_kernel(NormArgs a) {
 #pragma unroll
     for (int u = 0; u < V; ++u) {
       const int c = threadIdx.x * 8 + u * step, left = a.h - c;
-      float db[8], gd[8];
+      float db[8], dw1[8], gd[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         e[u][i] = __builtin_fmaf(-m, yh[u][i], e[u][i]);   // Dy
-        const float s_dy = a.scale * e[u][i];
         const float dp = token * sg[u][i] * e[u][i];
-        d1[u][i] = __builtin_fmaf(dp, bh[u][i], d1[u][i]);
-        gd[i] = s_dy * bh[u][i] * w1[u][i];
-        dg[u][i] += gd[i];
+        dw1[i] = dp * bh[u][i];
+        gd[i] = a.scale * e[u][i] * bh[u][i] * w1[u][i];
         db[i] = a.post ? i1 * (dp * w1[u][i] - bh[u][i] * mb) : dp;
       }
       if (a.d_block) store8<T>(a.d_block, base + c, left, db);
@@ -266,16 +307,24 @@ __global__ __launch_bounds__(NT) void gated_norm_backward_kernel(NormArgs a) {
         if (a.param_fp32 & 2) store8<Fp32>(a.d_gate, base + c, left, gd);
         else store8<T>(a.d_gate, base + c, left, gd);
       }
+      if (a.want_post) add(0, u, dw1);
+      if (a.want_gate) add(2, u, gd);
     }
   }
   float* plane = a.planes + (int64_t)blockIdx.x * (a.want_post + a.want_pre + a.want_gate) * a.h;
+  int64_t o = 0;
 #pragma unroll
-  for (int u = 0; u < V; ++u) {
-    const int c = threadIdx.x * 8 + u * step, left = a.h - c;
-    int64_t o = c;
-    if (a.want_post) { store8<Fp32>(plane, o, left, d1[u]); o += a.h; }
-    if (a.want_pre) { store8<Fp32>(plane, o, left, d2[u]); o += a.h; }
-    if (a.want_gate) store8<Fp32>(plane, o, left, dg[u]);
+  for (int kind = 0; kind < 3; ++kind) {
+    if (!(kind == 0 ? a.want_post : kind == 1 ? a.want_pre : a.want_gate)) continue;
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      const int c = threadIdx.x * 8 + u * step, left = a.h - c;
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = ACC_LDS ? s_acc[kind * step + threadIdx.x * 8 + i] : racc[ACC_LDS ? 0 : kind][u][i];
+      store8<Fp32>(plane, o + c, left, v);
+    }
+    o += a.h;
   }
 }
 
@@ -293,6 +342,7 @@ __global__ __launch_bounds__(1024) void plane_sum_kernel(SumArgs a) {
   const int64_t col = (int64_t)blockIdx.x * 64 + lane, cols = (int64_t)a.kinds * a.h;
   float s = 0.0f;
   if (col < cols)
+#pragma unroll 8
     for (int b = wave; b < a.blocks; b += 16) s += a.planes[(int64_t)b * cols + col];
   s_part[wave][lane] = s;
   __syncthreads();
@@ -306,39 +356,58 @@ __global__ __launch_bounds__(1024) void plane_sum_kernel(SumArgs a) {
   else store_one<T>(reinterpret_cast<uint8_t*>(a.out[kind]) + c * T::kBytes, s);
 }
 
-extern "C" { __attribute__((visibility("default"))) int bgmoe_n_force = 2; __attribute__((visibility("default"))) int bgmoe_nb_force = 1024; }
-// threads per row and vectors per thread: one vector up to 8192 columns, two above
-int threads_for(int h, int* vecs) {
-  *vecs = h > 8192 ? 2 : bgmoe_n_force;
-  return ((h + 8 * *vecs - 1) / (8 * *vecs) + BGMOE_WAVE - 1) / BGMOE_WAVE * BGMOE_WAVE;
-}
-// blocks of the gradient pass: enough to fill the chip (2048 threads per CU), each walking many rows
+// Threads for rows of h elements in `vecs` vectors of eight.
+int threads_for(int h, int vecs) { return ((h + 8 * vecs - 1) / (8 * vecs) + BGMOE_WAVE - 1) / BGMOE_WAVE * BGMOE_WAVE; }
+// Forward: two vectors per thread from 1024 rows on (half the waves per row: more rows at work; with the int8 form
+// 16384 x 7168 269 us against 340, 4096 x 7168 45 against 54 us without it), one below (a shorter chain per row: 16 x
+// 7168 5.4 against 5.9 us, 333 x 1001 5.4 against 6.9).  16384 x 7168 bf16: 230 us, 4.1 TB/s.
+int forward_vecs(int64_t rows, int h) { return h > 8192 || rows >= 1024 ? 2 : 1; }
+int backward_vecs(int h) { return h > 8192 ? 2 : 1; }
+// Blocks of the gradient pass: what is resident at 128 registers per thread (1024 threads per CU), at most one per row.
+// Fewer blocks would write fewer planes, but a row takes a block about 2.2 us: 1024 x 7168 35 us with 256 blocks, 82
+// with 64; 4096 x 2048 56 us with 256.  16384 x 7168 bf16: 361 us, 3.9 TB/s.
 int64_t backward_blocks(int64_t rows, int h) {
-  int vecs;
-  const int threads = threads_for(h, &vecs);
-  int64_t blocks = 256 * (2048 / threads);
-  if (blocks > bgmoe_nb_force) blocks = bgmoe_nb_force;
+  const int64_t blocks = 256 * (1024 / threads_for(h, backward_vecs(h)));
   return rows < blocks ? rows : blocks;
 }
 
 template <typename T>
 int run_forward(const NormArgs& a, hipStream_t st) {
-  int vecs;
-  const int threads = threads_for(a.h, &vecs);
+  const int vecs = forward_vecs(a.rows, a.h), threads = threads_for(a.h, vecs);
   BgmoeProf prof(BGMOE_K_GATED_NORM, st);
   if (vecs == 1) hipLaunchKernelGGL((gated_norm_kernel<T, 1>), bgmoe_grid(a.rows), dim3(threads), 0, st, a);
-  else if (vecs == 4) hipLaunchKernelGGL((gated_norm_kernel<T, 4>), bgmoe_grid(a.rows), dim3(threads), 0, st, a);
   else hipLaunchKernelGGL((gated_norm_kernel<T, 2>), bgmoe_grid(a.rows), dim3(threads), 0, st, a);
   return bgmoe_check_launch("gated_residual_norm");
 }
+// the dynamic-LDS opt-in (more than 64 KB), once per device
+int ensure_init() {
+  static bool done[64] = {};
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) {
+    bgmoe_set_error("gated_residual_norm_backward: no current HIP device (or device index >= 64)");
+    return BGMOE_ERR_HIP;
+  }
+  if (done[dev]) return BGMOE_OK;
+  const void* fns[3] = {(const void*)gated_norm_backward_kernel<Bf16, 1, true>, (const void*)gated_norm_backward_kernel<Fp16, 1, true>,
+                        (const void*)gated_norm_backward_kernel<Fp32, 1, true>};
+  for (const void* f : fns) {
+    const hipError_t err = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 1024 * kAccBytes);
+    if (err != hipSuccess) {
+      bgmoe_set_error("gated_residual_norm_backward: hipFuncSetAttribute(dynamic LDS) failed: %s", hipGetErrorString(err));
+      return BGMOE_ERR_HIP;
+    }
+  }
+  done[dev] = true;
+  return BGMOE_OK;
+}
 template <typename T>
 int run_backward(const NormArgs& a, const SumArgs& s, hipStream_t st) {
-  int vecs;
-  const int threads = threads_for(a.h, &vecs);
+  const int rc = ensure_init();
+  if (rc != BGMOE_OK) return rc;
+  const int vecs = backward_vecs(a.h), threads = threads_for(a.h, vecs);
   BgmoeProf prof(BGMOE_K_GATED_NORM, st);
-  if (vecs == 1) hipLaunchKernelGGL((gated_norm_backward_kernel<T, 1, 1024>), dim3((unsigned)s.blocks), dim3(threads), 0, st, a);
-  else if (threads <= 512) hipLaunchKernelGGL((gated_norm_backward_kernel<T, 2, 512>), dim3((unsigned)s.blocks), dim3(threads), 0, st, a);
-  else hipLaunchKernelGGL((gated_norm_backward_kernel<T, 2, 1024>), dim3((unsigned)s.blocks), dim3(threads), 0, st, a);
+  if (vecs == 1) hipLaunchKernelGGL((gated_norm_backward_kernel<T, 1, true>), dim3((unsigned)s.blocks), dim3(threads), threads * kAccBytes, st, a);
+  else hipLaunchKernelGGL((gated_norm_backward_kernel<T, 2, false>), dim3((unsigned)s.blocks), dim3(threads), 0, st, a);
   if (s.kinds) {
     const int64_t cols = (int64_t)s.kinds * s.h;
     hipLaunchKernelGGL((plane_sum_kernel<T>), dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, st, s);
@@ -358,6 +427,8 @@ int check_common(const char* what, int dtype, const void* gate, int gate_mode, i
 }
 
 }  // namespace
+
+int bgmoe_internal_init_gated_norm() { return ensure_init(); }
 
 extern "C" int bgmoe_gated_residual_norm(const void* block, const void* residual, int dtype, const void* post_weight,
                                          const void* gate, int gate_mode, float residual_scale, const void* pre_weight,

@@ -33,6 +33,7 @@ extern "C" int bgmoe_init(void) {
   if (rc == BGMOE_OK) rc = bgmoe_internal_init_router_gemm();
   if (rc == BGMOE_OK) rc = bgmoe_internal_init_permute();
   if (rc == BGMOE_OK) rc = bgmoe_internal_init_int8_gemm();
+  if (rc == BGMOE_OK) rc = bgmoe_internal_init_gated_norm();
   return rc;
 }
 
