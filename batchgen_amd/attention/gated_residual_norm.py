@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from .._lib import check, lib, ptr, stream
+from .._lib import lib, ptr
 from ..kernels import _checks as ck
 from ..quantization.int8 import no_grad_needed
 
@@ -67,11 +67,40 @@ class _Call:
 
 def _forward(c, block, residual, post, gate, pre, y, normed, q, q_scale, inv_post, inv_pre):
     if c.rows:
-        with torch.cuda.device(c.device):
-            check(lib().bgmoe_gated_residual_norm(ptr(block), ptr(residual), c.code, ptr(post), ptr(gate), c.gate_mode,
-                                                  c.scale, ptr(pre), c.param_fp32, c.rows, c.h, c.eps, ptr(y),
-                                                  ptr(normed), ptr(q), ptr(q_scale), ptr(inv_post), ptr(inv_pre),
-                                                  stream()))
+        ck.launch(c.device, lib().bgmoe_gated_residual_norm, ptr(block), ptr(residual), c.code, ptr(post), ptr(gate),
+                  c.gate_mode, c.scale, ptr(pre), c.param_fp32, c.rows, c.h, c.eps, ptr(y), ptr(normed), ptr(q),
+                  ptr(q_scale), inv_post, inv_pre)
+
+
+def _backward(ctx, d_y, d_normed):
+    block, residual, post, gate, pre, inv = ctx.saved_tensors
+    c, need = ctx.call, ctx.needs_input_grad
+    if d_y is None and d_normed is None:
+        return None, None, None, None, None, None
+    grads = [torch.empty_like(t) if t is not None and need[i] else None
+             for i, t in enumerate((block, residual, post, gate, pre))]
+    d_block, d_residual, d_post, d_gate, d_pre = grads
+    if c.rows == 0:
+        for g in grads:
+            if g is not None:
+                g.zero_()
+        return (*grads, None)
+    d_y = None if d_y is None else d_y.contiguous()
+    d_normed = None if d_normed is None else d_normed.contiguous()
+    nbytes = 0
+    if d_post is not None or d_pre is not None or (d_gate is not None and c.gate_mode == _CHANNEL):
+        nbytes = int(lib().bgmoe_gated_residual_norm_backward_workspace_bytes(c.rows, c.h))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=c.device) if nbytes else None
+    ck.launch(c.device, lib().bgmoe_gated_residual_norm_backward, ptr(block), ptr(residual), c.code, ptr(post),
+              ptr(gate), c.gate_mode, c.scale, ptr(pre), c.param_fp32, c.rows, c.h, ptr(inv), ptr(inv) + 4 * c.rows,
+              ptr(d_y), ptr(d_normed), ptr(d_block), ptr(d_residual), ptr(d_post), ptr(d_gate), ptr(d_pre), ptr(ws),
+              nbytes)
+    return (*grads, None)
+
+
+# The gradient has none of its own.  once_differentiable says so where it matters, but costs 75 us a call: it wraps it
+# only while a graph of the backward pass is being recorded.
+_backward_once = once_differentiable(_backward)
 
 
 class _GatedNorm(torch.autograd.Function):
@@ -81,38 +110,15 @@ class _GatedNorm(torch.autograd.Function):
         y = torch.empty_like(block)
         normed = torch.empty_like(block) if pre is not None else None
         inv = torch.empty((2, call.rows), dtype=torch.float32, device=call.device)
-        _forward(call, block, residual, post, gate, pre, y, normed, None, None, inv[0], inv[1])
+        _forward(call, block, residual, post, gate, pre, y, normed, None, None, inv.data_ptr(),
+                 inv.data_ptr() + 4 * call.rows)
         ctx.call = call
         ctx.save_for_backward(block, residual, post, gate, pre, inv)
         return y, normed
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_y, d_normed):
-        block, residual, post, gate, pre, inv = ctx.saved_tensors
-        c, need = ctx.call, ctx.needs_input_grad
-        if d_y is None and d_normed is None:
-            return None, None, None, None, None, None
-        new = lambda t, i: torch.empty_like(t) if t is not None and need[i] else None      # noqa: E731
-        grads = [new(t, i) for i, t in enumerate((block, residual, post, gate, pre))]
-        d_block, d_residual, d_post, d_gate, d_pre = grads
-        if c.rows == 0:
-            for g in grads:
-                if g is not None:
-                    g.zero_()
-            return (*grads, None)
-        d_y = None if d_y is None else d_y.contiguous()
-        d_normed = None if d_normed is None else d_normed.contiguous()
-        nbytes = 0
-        if d_post is not None or d_pre is not None or (d_gate is not None and c.gate_mode == _CHANNEL):
-            nbytes = int(lib().bgmoe_gated_residual_norm_backward_workspace_bytes(c.rows, c.h))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=c.device) if nbytes else None
-        with torch.cuda.device(c.device):
-            check(lib().bgmoe_gated_residual_norm_backward(
-                ptr(block), ptr(residual), c.code, ptr(post), ptr(gate), c.gate_mode, c.scale, ptr(pre), c.param_fp32,
-                c.rows, c.h, ptr(inv[0]), ptr(inv[1]), ptr(d_y), ptr(d_normed), ptr(d_block), ptr(d_residual),
-                ptr(d_post), ptr(d_gate), ptr(d_pre), ptr(ws), nbytes, stream()))
-        return (*grads, None)
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, d_y, d_normed)
 
 
 def _contiguous(*tensors):

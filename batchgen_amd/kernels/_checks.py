@@ -4,6 +4,11 @@ from __future__ import annotations
 
 import torch
 
+from .._lib import check
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
 
 def fail(msg: str):
     raise RuntimeError(msg)
@@ -58,6 +63,17 @@ def combine_args(expert_output, topk_pos, topk_weights, output, n, h, k, out_dty
 
 
 FP8_BYTES = (torch.uint8, torch.float8_e4m3fn)
+
+def launch(device: torch.device, fn, *args):
+    """``fn(*args, stream)`` with ``device`` current, on its current stream.  The context manager and the stream object of
+    torch.cuda take 4 us, as much as a short kernel; where the device is the current one already neither is needed."""
+    index = device.index
+    if index == _current_device():
+        check(fn(*args, _raw_stream(index)))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _raw_stream(index)))
+
 
 # BGMOE_DT_*: element types of the operators that take all three
 DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}

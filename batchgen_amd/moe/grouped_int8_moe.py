@@ -14,7 +14,7 @@ from typing import Optional
 
 import torch
 
-from .._lib import check, lib, ptr, stream
+from .._lib import lib, ptr
 from ..kernels import _checks as ck
 from ..quantization.int8 import no_grad_needed
 
@@ -75,10 +75,9 @@ def int8_grouped_gemm(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tens
     n = weight.size(1)
     out, code = _out(x, out, out_dtype, m, n)
     if m and n:
-        with torch.cuda.device(x.device):
-            check(lib().bgmoe_int8_grouped_gemm(ptr(x), ptr(x_scale), ptr(weight), weight.stride(0), ptr(weight_scale),
-                                                weight_scale.stride(0), ptr(seqlens), ptr(cu_seqlens), e, m, n, k,
-                                                ptr(out), code, stream()))
+        ck.launch(x.device, lib().bgmoe_int8_grouped_gemm, ptr(x), ptr(x_scale), ptr(weight), weight.stride(0),
+                  ptr(weight_scale), weight_scale.stride(0), ptr(seqlens), ptr(cu_seqlens), e, m, n, k, ptr(out),
+                  code)
     return out
 
 
@@ -97,9 +96,7 @@ def int8_fused_s1(x: torch.Tensor, x_scale: torch.Tensor, gate_weight: torch.Ten
     n = gate_weight.size(1)
     out, code = _out(x, out, out_dtype, m, n)
     if m and n:
-        with torch.cuda.device(x.device):
-            check(lib().bgmoe_int8_fused_s1(ptr(x), ptr(x_scale), ptr(gate_weight), gate_weight.stride(0),
-                                            ptr(gate_scale), gate_scale.stride(0), ptr(up_weight), up_weight.stride(0),
-                                            ptr(up_scale), up_scale.stride(0), ptr(seqlens), ptr(cu_seqlens), e, m, n, k,
-                                            ptr(out), code, stream()))
+        ck.launch(x.device, lib().bgmoe_int8_fused_s1, ptr(x), ptr(x_scale), ptr(gate_weight), gate_weight.stride(0),
+                  ptr(gate_scale), gate_scale.stride(0), ptr(up_weight), up_weight.stride(0), ptr(up_scale),
+                  up_scale.stride(0), ptr(seqlens), ptr(cu_seqlens), e, m, n, k, ptr(out), code)
     return out

@@ -19,7 +19,7 @@ from typing import Optional
 import torch
 from torch.autograd.function import once_differentiable
 
-from .._lib import check, lib, ptr, stream
+from .._lib import lib, ptr
 from ..kernels import _checks as ck
 from .dispatch_scatter_3d import ragged_row_capacity
 
@@ -54,9 +54,8 @@ def token_sort_plan(topk_ids: torch.Tensor, num_experts: int, expert_start: int 
     pos = torch.empty((n, k), dtype=torch.int32, device=dev)
     need = int(lib().bgmoe_dispatch_workspace_bytes(n * k, e))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with torch.cuda.device(dev):
-        check(lib().bgmoe_token_sort_index(ptr(ids), int(ids.dtype == torch.int64), n, k, int(expert_start), e, row_align,
-                                           ptr(meta), ptr(meta) + 4 * e, ptr(pos), ptr(ws), need, stream()))
+    ck.launch(dev, lib().bgmoe_token_sort_index, ptr(ids), int(ids.dtype == torch.int64), n, k, int(expert_start), e,
+              row_align, ptr(meta), ptr(meta) + 4 * e, ptr(pos), ptr(ws), need)
     return TokenSortPlan(meta[:e], meta[e:], pos, e, row_align, ragged_row_capacity(n, k, e, row_align))
 
 
@@ -81,10 +80,9 @@ def _run_sort(x, plan, out):
     if out is None:
         out = torch.empty((plan.capacity, h), dtype=x.dtype, device=x.device)
     size = x.element_size()
-    with torch.cuda.device(x.device):
-        check(lib().bgmoe_token_sort_rows(ptr(x), x.stride(0) * size, h * size, plan.num_tokens, plan.top_k,
-                                          ptr(plan.topk_pos), ptr(plan.counts), ptr(plan.cu_seqlens), plan.num_experts,
-                                          plan.capacity, int(zero_rest), ptr(out), stream()))
+    ck.launch(x.device, lib().bgmoe_token_sort_rows, ptr(x), x.stride(0) * size, h * size, plan.num_tokens,
+              plan.top_k, ptr(plan.topk_pos), ptr(plan.counts), ptr(plan.cu_seqlens), plan.num_experts, plan.capacity,
+              int(zero_rest), ptr(out))
     return out
 
 
@@ -92,10 +90,31 @@ def _run_unsort(rows, plan, weights, out):
     h = rows.size(1)
     if out is None:
         out = torch.empty((plan.num_tokens, h), dtype=rows.dtype, device=rows.device)
-    with torch.cuda.device(rows.device):
-        check(lib().bgmoe_token_unsort(ptr(rows), ck.dtype_code(rows, "rows"), ptr(plan.topk_pos), ptr(weights),
-                                       plan.num_tokens, plan.top_k, h, ptr(out), stream()))
+    ck.launch(rows.device, lib().bgmoe_token_unsort, ptr(rows), ck.dtype_code(rows, "rows"), ptr(plan.topk_pos),
+              ptr(weights), plan.num_tokens, plan.top_k, h, ptr(out))
     return out
+
+
+# The gradients have none of their own.  once_differentiable says so where it matters, but costs 75 us a call: it wraps
+# them only while a graph of the backward pass is being recorded.
+def _sort_backward(ctx, d_rows):
+    return _run_unsort(d_rows.contiguous(), ctx.plan, None, None), None
+
+
+def _unsort_backward(ctx, d_out):
+    rows, weights = ctx.saved_tensors
+    plan, d_out = ctx.plan, d_out.contiguous()
+    d_rows = torch.empty_like(rows) if ctx.needs_input_grad[0] else None
+    d_weights = torch.empty_like(weights) if weights is not None and ctx.needs_input_grad[1] else None
+    if d_rows is not None or d_weights is not None:
+        ck.launch(rows.device, lib().bgmoe_token_unsort_backward, ptr(d_out), ptr(rows), ck.dtype_code(rows, "rows"),
+                  ptr(plan.topk_pos), ptr(weights), plan.num_tokens, plan.top_k, rows.size(1), ptr(plan.counts),
+                  ptr(plan.cu_seqlens), plan.num_experts, plan.capacity, ptr(d_rows), ptr(d_weights))
+    return d_rows, d_weights, None
+
+
+_sort_backward_once = once_differentiable(_sort_backward)
+_unsort_backward_once = once_differentiable(_unsort_backward)
 
 
 class _Sort(torch.autograd.Function):
@@ -105,9 +124,8 @@ class _Sort(torch.autograd.Function):
         return _run_sort(x, plan, None)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_rows):
-        return _run_unsort(d_rows.contiguous(), ctx.plan, None, None), None
+        return (_sort_backward_once if torch.is_grad_enabled() else _sort_backward)(ctx, d_rows)
 
 
 class _Unsort(torch.autograd.Function):
@@ -118,19 +136,8 @@ class _Unsort(torch.autograd.Function):
         return _run_unsort(rows, plan, weights, None)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_out):
-        rows, weights = ctx.saved_tensors
-        plan, d_out = ctx.plan, d_out.contiguous()
-        d_rows = torch.empty_like(rows) if ctx.needs_input_grad[0] else None
-        d_weights = torch.empty_like(weights) if weights is not None and ctx.needs_input_grad[1] else None
-        if d_rows is not None or d_weights is not None:
-            with torch.cuda.device(rows.device):
-                check(lib().bgmoe_token_unsort_backward(
-                    ptr(d_out), ptr(rows), ck.dtype_code(rows, "rows"), ptr(plan.topk_pos), ptr(weights), plan.num_tokens,
-                    plan.top_k, rows.size(1), ptr(plan.counts), ptr(plan.cu_seqlens), plan.num_experts, plan.capacity,
-                    ptr(d_rows), ptr(d_weights), stream()))
-        return d_rows, d_weights, None
+        return (_unsort_backward_once if torch.is_grad_enabled() else _unsort_backward)(ctx, d_out)
 
 
 def sort_tokens(x: torch.Tensor, plan: TokenSortPlan, out: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -13,7 +13,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from .._lib import check, lib, ptr, stream
+from .._lib import lib, ptr
 from ..kernels import _checks as ck
 
 
@@ -45,8 +45,7 @@ def int8_quant_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
     if rows and k == 0:
         ck.fail("int8_quant_rows: rows without elements have no scale")
     if rows:
-        with torch.cuda.device(x.device):
-            check(lib().bgmoe_int8_quant_rows(ptr(x2), code, x2.stride(0), rows, k, ptr(out), ptr(scale), stream()))
+        ck.launch(x.device, lib().bgmoe_int8_quant_rows, ptr(x2), code, x2.stride(0), rows, k, ptr(out), ptr(scale))
     return out, scale
 
 
@@ -98,16 +97,13 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         if x2.data_ptr() % 16 or x2.stride(0) % 16:
             x2 = x2.contiguous() if x2.stride(0) % 16 else x2.clone()
         ws = _workspace(lib().bgmoe_int8_gemm_workspace_bytes(m, n, k), x.device)
-        with torch.cuda.device(x.device):
-            check(lib().bgmoe_int8_gemm(ptr(x2), x2.stride(0) if m > 1 else k, ptr(x_scale), ptr(weight),
-                                        ptr(weight_scale), ptr(bias), m, n, k, ptr(out), code, n, ptr(ws),
-                                        0 if ws is None else ws.numel(), stream()))
+        ck.launch(x.device, lib().bgmoe_int8_gemm, ptr(x2), x2.stride(0) if m > 1 else k, ptr(x_scale), ptr(weight),
+                  ptr(weight_scale), ptr(bias), m, n, k, ptr(out), code, n, ptr(ws), 0 if ws is None else ws.numel())
     else:
         x_code = ck.dtype_code(x, "x")
         ws = _workspace(lib().bgmoe_int8_linear_workspace_bytes(m, n, k), x.device)
-        with torch.cuda.device(x.device):
-            check(lib().bgmoe_int8_linear(ptr(x2), x_code, x2.stride(0), ptr(weight), ptr(weight_scale), ptr(bias), m, n,
-                                          k, ptr(out), code, n, ptr(ws), ws.numel(), stream()))
+        ck.launch(x.device, lib().bgmoe_int8_linear, ptr(x2), x_code, x2.stride(0), ptr(weight), ptr(weight_scale),
+                  ptr(bias), m, n, k, ptr(out), code, n, ptr(ws), ws.numel())
     return out
 
 

@@ -122,6 +122,9 @@ def run_package_on_emulator(monkeypatch):
             _checks.fail(f"{name} must be a tensor")
     monkeypatch.setattr(_checks, "gpu", tensor_only)
 
+    monkeypatch.setattr(_checks, "_current_device", lambda: None)
+    monkeypatch.setattr(_checks, "_raw_stream", lambda index: None)
+
     from batchgen_amd.kernels import _workspace
     pool = {}
 

@@ -242,6 +242,17 @@ def test_forward_and_backward_in_a_graph(dev):
                 assert torch.equal(a, b)
 
 
+def test_no_second_gradient(dev):
+    b, r, p, g, w = [t.clone().to(dev).requires_grad_(True) for t in operands(4, 24, torch.float32, "channel")]
+    y, n = api().gated_residual_rmsnorm(b, r, post_weight=p, gate=g, pre_weight=w)
+    first = torch.autograd.grad((y.sum(), n.square().sum()), (b, p), create_graph=True)
+    y, n = api().gated_residual_rmsnorm(b, r, post_weight=p, gate=g, pre_weight=w)
+    plain = torch.autograd.grad((y.sum(), n.square().sum()), (b, p))
+    assert all(torch.equal(u, v) for u, v in zip(first, plain))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first[0].sum(), b)
+
+
 def test_refusals(dev):
     f, q = api().gated_residual_rmsnorm, api().gated_residual_rmsnorm_int8_quant
     b, r, p, g, w = to(dev, *operands(4, 24, torch.bfloat16, "channel"))

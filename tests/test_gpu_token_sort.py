@@ -253,6 +253,21 @@ def test_forward_and_backward_in_a_graph(dev):
             assert torch.equal(a, b)
 
 
+def test_no_second_gradient(dev):
+    """A gradient of a gradient is refused where it is asked for, not answered with a wrong one."""
+    ids = make_ids(6, 2, 4, torch.int64, 31).to(dev)
+    plan = api().token_sort_plan(ids, 4)
+    x = rand(32, 6, 8).clone().to(dev).requires_grad_(True)
+    w = torch.rand(6, 2).to(dev).requires_grad_(True)
+    out = api().unsort_tokens(api().sort_tokens(x, plan), plan, w)
+    gx, gw = torch.autograd.grad(out.square().sum(), (x, w), create_graph=True)
+    plain = torch.autograd.grad(api().unsort_tokens(api().sort_tokens(x, plan), plan, w).square().sum(), (x, w))
+    assert torch.equal(gx, plain[0]) and torch.equal(gw, plain[1])
+    for g in (gx, gw):
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), x, retain_graph=True)
+
+
 def test_refusals(dev):
     t = api()
     ids = torch.zeros(4, 2, dtype=torch.int32, device=dev)
