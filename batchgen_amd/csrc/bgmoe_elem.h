@@ -13,6 +13,17 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 __device__ __forceinline__ u32x4 load16(const void* p) { return *reinterpret_cast<const u32x4_any*>(p); }
 __device__ __forceinline__ void store16(void* p, u32x4 v) { *reinterpret_cast<u32x4_any*>(p) = v; }
+// NT: past the last-level cache (256 MB), for data that does not fit there and is touched once
+template <bool NT>
+__device__ __forceinline__ u32x4 load16_as(const void* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+  else return load16(p);
+}
+template <bool NT>
+__device__ __forceinline__ void store16_as(void* p, u32x4 v) {
+  if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(p));
+  else store16(p, v);
+}
 
 template <typename T> constexpr int kPer16 = 16 / T::kBytes;      // elements in 16 bytes
 
@@ -81,13 +92,13 @@ __device__ __forceinline__ void load8(const void* row, int64_t c, int left, floa
 }
 // the same, still packed: half the registers for the two-byte types
 template <typename T> struct Packed8 { u32x4 v[T::kBytes / 2]; };
-template <typename T>
+template <typename T, bool NT = false>
 __device__ __forceinline__ Packed8<T> load8_packed(const void* row, int64_t c, int left) {
   const uint8_t* p = reinterpret_cast<const uint8_t*>(row) + c * T::kBytes;
   Packed8<T> r;
   if (left >= 8) {
-    r.v[0] = load16(p);
-    if constexpr (T::kBytes == 4) r.v[1] = load16(p + 16);
+    r.v[0] = load16_as<NT>(p);
+    if constexpr (T::kBytes == 4) r.v[1] = load16_as<NT>(p + 16);
   } else {
     typename T::raw e[8];
 #pragma unroll
@@ -101,12 +112,12 @@ __device__ __forceinline__ void unpack8(const Packed8<T>& r, float (&v)[8]) {
   unpack16<T>(r.v[0], v);
   if constexpr (T::kBytes == 4) unpack16<T>(r.v[1], v + 4);
 }
-template <typename T>
+template <typename T, bool NT = false>
 __device__ __forceinline__ void store8(void* row, int64_t c, int left, const float (&v)[8]) {
   uint8_t* p = reinterpret_cast<uint8_t*>(row) + c * T::kBytes;
   if (left >= 8) {
-    store16(p, pack16<T>(v));
-    if constexpr (T::kBytes == 4) store16(p + 16, pack16<T>(v + 4));
+    store16_as<NT>(p, pack16<T>(v));
+    if constexpr (T::kBytes == 4) store16_as<NT>(p + 16, pack16<T>(v + 4));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)

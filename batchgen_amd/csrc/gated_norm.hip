@@ -101,7 +101,7 @@ __device__ __forceinline__ float block_max(float v, float* buf) {
 __device__ __forceinline__ float inv_rms(float sum, int h, float eps) { return 1.0f / sqrtf(sum / (float)h + eps); }
 
 // One block per row, V vectors of eight elements per thread.
-template <typename T, int V>
+template <typename T, int V, bool NT>
 __global__ __launch_bounds__(1024) void gated_norm_kernel(NormArgs a) {
   __shared__ float s_sum[2][16][1];
   __shared__ float s_max[16];
@@ -114,8 +114,8 @@ __global__ __launch_bounds__(1024) void gated_norm_kernel(NormArgs a) {
 #pragma unroll
   for (int u = 0; u < V; ++u) {
     const int c = threadIdx.x * 8 + u * step, left = a.h - c;
-    load8<T>(a.block, base + c, left, b[u]);
-    load8<T>(a.residual, base + c, left, y[u]);
+    unpack8<T>(load8_packed<T, NT>(a.block, base + c, left), b[u]);
+    unpack8<T>(load8_packed<T, NT>(a.residual, base + c, left), y[u]);
   }
   if (a.post) {
     float sum[1] = {0.0f};
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(1024) void gated_norm_kernel(NormArgs a) {
     load_gate8<T>(a, row, c, left, token, g);
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[u][i] = __builtin_fmaf(g[i], b[u][i], y[u][i]);
-    store8<T>(a.y, base + c, left, y[u]);
+    store8<T, NT>(a.y, base + c, left, y[u]);
     if (left < 8)                                        // what lies past the row does not count
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[u][i] = i < left ? y[u][i] : 0.0f;
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(1024) void gated_norm_kernel(NormArgs a) {
     load_param8<T>(a.pre, (a.param_fp32 & 4) != 0, c, left, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[u][i] = y[u][i] * i2 * w[i];
-    if (a.normed) store8<T>(a.normed, base + c, left, y[u]);
+    if (a.normed) store8<T, NT>(a.normed, base + c, left, y[u]);
     if (a.q) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(1024) void gated_norm_kernel(NormArgs a) {
 // works on another.  What the blocks sum over their rows lives in LDS, eight floats per thread and kind (in registers it
 // takes the place of that next row, or of a second block per CU).  Order of the planes: post, pre, gate.
 // ACC_LDS = false (rows wider than LDS holds, h > 8192): accumulators in registers.
-template <typename T, int V, bool ACC_LDS>
+template <typename T, int V, bool ACC_LDS, bool NT>
 __global__ __launch_bounds__(1024) void gated_norm_backward_kernel(NormArgs a) {
   extern __shared__ __align__(16) float s_acc[];         // [kind][thread * 8 + i]
   __shared__ float s_sum[2][16][3];
@@ -229,10 +229,10 @@ __global__ __launch_bounds__(1024) void gated_norm_backward_kernel(NormArgs a) {
 #pragma unroll
     for (int u = 0; u < V; ++u) {
       const int c = threadIdx.x * 8 + u * step, left = a.h - c;
-      o.b[u] = load8_packed<T>(a.block, base + c, left);
-      o.r[u] = load8_packed<T>(a.residual, base + c, left);
-      o.dy[u] = a.dy ? load8_packed<T>(a.dy, base + c, left) : Packed8<T>{};
-      o.dn[u] = norm ? load8_packed<T>(a.dn, base + c, left) : Packed8<T>{};
+      o.b[u] = load8_packed<T, NT>(a.block, base + c, left);
+      o.r[u] = load8_packed<T, NT>(a.residual, base + c, left);
+      o.dy[u] = a.dy ? load8_packed<T, NT>(a.dy, base + c, left) : Packed8<T>{};
+      o.dn[u] = norm ? load8_packed<T, NT>(a.dn, base + c, left) : Packed8<T>{};
     }
     return o;
   };
@@ -301,8 +301,8 @@ __global__ __launch_bounds__(1024) void gated_norm_backward_kernel(NormArgs a) {
         gd[i] = a.scale * e[u][i] * bh[u][i] * w1[u][i];
         db[i] = a.post ? i1 * (dp * w1[u][i] - bh[u][i] * mb) : dp;
       }
-      if (a.d_block) store8<T>(a.d_block, base + c, left, db);
-      if (a.d_residual) store8<T>(a.d_residual, base + c, left, e[u]);
+      if (a.d_block) store8<T, NT>(a.d_block, base + c, left, db);
+      if (a.d_residual) store8<T, NT>(a.d_residual, base + c, left, e[u]);
       if (a.gate_mode == BGMOE_GATE_FULL && a.d_gate) {
         if (a.param_fp32 & 2) store8<Fp32>(a.d_gate, base + c, left, gd);
         else store8<T>(a.d_gate, base + c, left, gd);
@@ -359,24 +359,31 @@ __global__ __launch_bounds__(1024) void plane_sum_kernel(SumArgs a) {
 // Threads for rows of h elements in `vecs` vectors of eight.
 int threads_for(int h, int vecs) { return ((h + 8 * vecs - 1) / (8 * vecs) + BGMOE_WAVE - 1) / BGMOE_WAVE * BGMOE_WAVE; }
 // Forward: two vectors per thread from 1024 rows on (half the waves per row: more rows at work; with the int8 form
-// 16384 x 7168 269 us against 340, 4096 x 7168 45 against 54 us without it), one below (a shorter chain per row: 16 x
-// 7168 5.4 against 5.9 us, 333 x 1001 5.4 against 6.9).  16384 x 7168 bf16: 230 us, 4.1 TB/s.
+// 16384 x 7168 269 us against 340 through the cache, 4096 x 7168 45 against 54 us without it), one below (a shorter chain per row: 16 x
+// 7168 5.4 against 5.9 us, 333 x 1001 5.4 against 6.9).
 int forward_vecs(int64_t rows, int h) { return h > 8192 || rows >= 1024 ? 2 : 1; }
 int backward_vecs(int h) { return h > 8192 ? 2 : 1; }
 // Blocks of the gradient pass: what is resident at 128 registers per thread (1024 threads per CU), at most one per row.
 // Fewer blocks would write fewer planes, but a row takes a block about 2.2 us: 1024 x 7168 35 us with 256 blocks, 82
-// with 64; 4096 x 2048 56 us with 256.  16384 x 7168 bf16: 361 us, 3.9 TB/s.
+// with 64; 4096 x 2048 56 us with 256.  16384 x 7168 bf16: 356 us, 4.0 TB/s.
 int64_t backward_blocks(int64_t rows, int h) {
   const int64_t blocks = 256 * (1024 / threads_for(h, backward_vecs(h)));
   return rows < blocks ? rows : blocks;
 }
 
+// Whether a pass over `operands` row matrices moves more than the last-level cache holds, which it then bypasses: forward
+// of 16384 x 7168 bf16 230 -> 168 us (5.6 TB/s), with the int8 form 269 -> 203, gradient 361 -> 356; gradient of 16384 x
+// 2048 116 -> 96 us.  4096 x 7168, which fits, 45.2 us through it and 47.5 past it.
+template <typename T>
+bool past_cache(const NormArgs& a, int operands) { return a.rows * a.h * T::kBytes * operands > (256LL << 20); }
+
 template <typename T>
 int run_forward(const NormArgs& a, hipStream_t st) {
   const int vecs = forward_vecs(a.rows, a.h), threads = threads_for(a.h, vecs);
   BgmoeProf prof(BGMOE_K_GATED_NORM, st);
-  if (vecs == 1) hipLaunchKernelGGL((gated_norm_kernel<T, 1>), bgmoe_grid(a.rows), dim3(threads), 0, st, a);
-  else hipLaunchKernelGGL((gated_norm_kernel<T, 2>), bgmoe_grid(a.rows), dim3(threads), 0, st, a);
+  if (vecs == 1) hipLaunchKernelGGL((gated_norm_kernel<T, 1, false>), bgmoe_grid(a.rows), dim3(threads), 0, st, a);
+  else if (!past_cache<T>(a, 4)) hipLaunchKernelGGL((gated_norm_kernel<T, 2, false>), bgmoe_grid(a.rows), dim3(threads), 0, st, a);
+  else hipLaunchKernelGGL((gated_norm_kernel<T, 2, true>), bgmoe_grid(a.rows), dim3(threads), 0, st, a);
   return bgmoe_check_launch("gated_residual_norm");
 }
 // the dynamic-LDS opt-in (more than 64 KB), once per device
@@ -388,8 +395,10 @@ int ensure_init() {
     return BGMOE_ERR_HIP;
   }
   if (done[dev]) return BGMOE_OK;
-  const void* fns[3] = {(const void*)gated_norm_backward_kernel<Bf16, 1, true>, (const void*)gated_norm_backward_kernel<Fp16, 1, true>,
-                        (const void*)gated_norm_backward_kernel<Fp32, 1, true>};
+  const void* fns[6] = {
+      (const void*)gated_norm_backward_kernel<Bf16, 1, true, false>, (const void*)gated_norm_backward_kernel<Bf16, 1, true, true>,
+      (const void*)gated_norm_backward_kernel<Fp16, 1, true, false>, (const void*)gated_norm_backward_kernel<Fp16, 1, true, true>,
+      (const void*)gated_norm_backward_kernel<Fp32, 1, true, false>, (const void*)gated_norm_backward_kernel<Fp32, 1, true, true>};
   for (const void* f : fns) {
     const hipError_t err = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 1024 * kAccBytes);
     if (err != hipSuccess) {
@@ -406,8 +415,10 @@ int run_backward(const NormArgs& a, const SumArgs& s, hipStream_t st) {
   if (rc != BGMOE_OK) return rc;
   const int vecs = backward_vecs(a.h), threads = threads_for(a.h, vecs);
   BgmoeProf prof(BGMOE_K_GATED_NORM, st);
-  if (vecs == 1) hipLaunchKernelGGL((gated_norm_backward_kernel<T, 1, true>), dim3((unsigned)s.blocks), dim3(threads), threads * kAccBytes, st, a);
-  else hipLaunchKernelGGL((gated_norm_backward_kernel<T, 2, false>), dim3((unsigned)s.blocks), dim3(threads), 0, st, a);
+  const dim3 grid((unsigned)s.blocks), block(threads);
+  if (vecs == 2) hipLaunchKernelGGL((gated_norm_backward_kernel<T, 2, false, false>), grid, block, 0, st, a);
+  else if (!past_cache<T>(a, 6)) hipLaunchKernelGGL((gated_norm_backward_kernel<T, 1, true, false>), grid, block, threads * kAccBytes, st, a);
+  else hipLaunchKernelGGL((gated_norm_backward_kernel<T, 1, true, true>), grid, block, threads * kAccBytes, st, a);
   if (s.kinds) {
     const int64_t cols = (int64_t)s.kinds * s.h;
     hipLaunchKernelGGL((plane_sum_kernel<T>), dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, st, s);
