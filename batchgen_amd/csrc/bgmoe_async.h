@@ -19,6 +19,11 @@ __device__ __forceinline__ void async_load16(const uint8_t* base, uint32_t lane_
   asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :: "s"(lds_base), "v"(lane_off), "s"(base) : "memory", "m0");
 }
+// The same past the last-level cache: operands that are read once.
+__device__ __forceinline__ void async_load16_nt(const uint8_t* base, uint32_t lane_off, uint32_t lds_base) {
+  asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+               :: "s"(lds_base), "v"(lane_off), "s"(base) : "memory", "m0");
+}
 // The same with a full address per lane, for lanes whose sources do not lie behind one base (a K tail whose missing
 // chunks read a block of zeros).
 __device__ __forceinline__ void async_load16_lane(const void* lane_ptr, uint32_t lds_base) {

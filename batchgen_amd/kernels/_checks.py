@@ -36,6 +36,10 @@ def dtype(t: torch.Tensor, dt, name: str):
 
 
 def cuda_tensor(ref, t, dt, name):
+    # one expression for the common case; the checks below say what is wrong otherwise
+    if isinstance(t, torch.Tensor) and t.dtype is dt and t.is_cuda and t.is_contiguous() and \
+            (ref is None or t.get_device() == ref.get_device()):
+        return
     gpu(t, name)
     if ref is not None:
         same_device(ref, t, name)
@@ -88,6 +92,8 @@ def dtype_code(t: torch.Tensor, name: str) -> int:
 
 def rows_of(t: torch.Tensor, name: str) -> torch.Tensor:
     """``t [..., K]`` as ``[rows, K]`` whose rows are contiguous (a 2-D tensor may keep a stride between its rows)."""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     if t.dim() == 0:
         fail(f"{name} must have at least one axis")
     if t.dim() == 2 and (t.stride(1) == 1 or t.size(1) <= 1) and (t.stride(0) >= t.size(1) or t.size(0) <= 1):

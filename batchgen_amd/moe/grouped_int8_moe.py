@@ -37,6 +37,9 @@ def _rows(x, x_scale, seqlens, cu_seqlens, e):
 
 def _weight(x, w, s, k, name):
     """Checks ``w [E, N, K]`` / ``s [E, N]`` (experts may be strided, e.g. halves of a stacked ``[E, 2N, K]``)."""
+    if w.dtype is torch.int8 and s.dtype is torch.float32 and w.is_contiguous() and s.is_contiguous() and w.dim() == 3 and \
+            w.size(2) == k and s.shape == w.shape[:2] and w.get_device() == s.get_device() == x.get_device():
+        return
     ck.gpu(w, name)
     ck.same_device(x, w, name)
     ck.dtype(w, torch.int8, name)

@@ -29,12 +29,20 @@ MAX_TOP_K = 32
 class TokenSortPlan:
     """``counts`` int32 ``[E]``, ``cu_seqlens`` int32 ``[E + 1]``, ``topk_pos`` int32 ``[N, K]`` (-1: no row), and the
     host-side sizes; ``capacity`` is the row count of a sorted buffer (enough for any routing)."""
-    __slots__ = ("counts", "cu_seqlens", "topk_pos", "num_tokens", "top_k", "num_experts", "row_align", "capacity")
+    __slots__ = ("meta", "topk_pos", "num_tokens", "top_k", "num_experts", "row_align", "capacity")
 
-    def __init__(self, counts, cu_seqlens, topk_pos, num_experts, row_align, capacity):
-        self.counts, self.cu_seqlens, self.topk_pos = counts, cu_seqlens, topk_pos
+    def __init__(self, meta, topk_pos, num_experts, row_align, capacity):
+        self.meta, self.topk_pos = meta, topk_pos          # meta: counts, then cu_seqlens
         self.num_tokens, self.top_k = topk_pos.shape
         self.num_experts, self.row_align, self.capacity = num_experts, row_align, capacity
+
+    @property
+    def counts(self) -> torch.Tensor:
+        return self.meta[:self.num_experts]
+
+    @property
+    def cu_seqlens(self) -> torch.Tensor:
+        return self.meta[self.num_experts:]
 
 
 def token_sort_plan(topk_ids: torch.Tensor, num_experts: int, expert_start: int = 0, row_align: int = 1) -> TokenSortPlan:
@@ -56,7 +64,7 @@ def token_sort_plan(topk_ids: torch.Tensor, num_experts: int, expert_start: int 
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     ck.launch(dev, lib().bgmoe_token_sort_index, ptr(ids), int(ids.dtype == torch.int64), n, k, int(expert_start), e,
               row_align, ptr(meta), ptr(meta) + 4 * e, ptr(pos), ptr(ws), need)
-    return TokenSortPlan(meta[:e], meta[e:], pos, e, row_align, ragged_row_capacity(n, k, e, row_align))
+    return TokenSortPlan(meta, pos, e, row_align, ragged_row_capacity(n, k, e, row_align))
 
 
 def _tokens(x, plan, name, rows):
@@ -81,7 +89,7 @@ def _run_sort(x, plan, out):
         out = torch.empty((plan.capacity, h), dtype=x.dtype, device=x.device)
     size = x.element_size()
     ck.launch(x.device, lib().bgmoe_token_sort_rows, ptr(x), x.stride(0) * size, h * size, plan.num_tokens,
-              plan.top_k, ptr(plan.topk_pos), ptr(plan.counts), ptr(plan.cu_seqlens), plan.num_experts, plan.capacity,
+              plan.top_k, ptr(plan.topk_pos), ptr(plan.meta), ptr(plan.meta) + 4 * plan.num_experts, plan.num_experts, plan.capacity,
               int(zero_rest), ptr(out))
     return out
 
@@ -108,8 +116,8 @@ def _unsort_backward(ctx, d_out):
     d_weights = torch.empty_like(weights) if weights is not None and ctx.needs_input_grad[1] else None
     if d_rows is not None or d_weights is not None:
         ck.launch(rows.device, lib().bgmoe_token_unsort_backward, ptr(d_out), ptr(rows), ck.dtype_code(rows, "rows"),
-                  ptr(plan.topk_pos), ptr(weights), plan.num_tokens, plan.top_k, rows.size(1), ptr(plan.counts),
-                  ptr(plan.cu_seqlens), plan.num_experts, plan.capacity, ptr(d_rows), ptr(d_weights))
+                  ptr(plan.topk_pos), ptr(weights), plan.num_tokens, plan.top_k, rows.size(1), ptr(plan.meta),
+                  ptr(plan.meta) + 4 * plan.num_experts, plan.num_experts, plan.capacity, ptr(d_rows), ptr(d_weights))
     return d_rows, d_weights, None
 
 

@@ -18,8 +18,10 @@ from ..kernels import _checks as ck
 
 
 def no_grad_needed(name: str, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        ck.fail(f"{name} has no gradient: call it under torch.no_grad() or detach its operands")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                ck.fail(f"{name} has no gradient: call it under torch.no_grad() or detach its operands")
 
 
 def int8_quant_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,

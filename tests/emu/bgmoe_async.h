@@ -18,6 +18,9 @@
 __device__ __forceinline__ void async_load16(const uint8_t* base, uint32_t lane_off, uint32_t lds_base) {
   emu::async_load(base, lane_off, lds_base, 16);
 }
+__device__ __forceinline__ void async_load16_nt(const uint8_t* base, uint32_t lane_off, uint32_t lds_base) {
+  emu::async_load(base, lane_off, lds_base, 16);
+}
 __device__ __forceinline__ void async_load16_lane(const void* lane_ptr, uint32_t lds_base) {
   emu::async_load(lane_ptr, 0, lds_base, 16, false);
 }
