@@ -157,3 +157,55 @@ def test_trainable_block(dev):
     d_x, d_res, d_post, d_pre, d_gate = torch.autograd.grad((ya, na), first, (d_y, d_n))
     for got, want in zip(whole, (d_x, d_res, d_post + d_post2, d_pre + d_pre2, d_gate, d_w, d_mats)):
         assert torch.equal(got, want) or torch.allclose(got, want, rtol=2 * ref.U32, atol=0)       # one sum of two terms
+
+
+@pytest.mark.skipif(emulating(), reason="tens of GB")
+def test_offsets_past_32_bits(dev):
+    """Operands of more than 2^32 bytes (and 2^31 elements): the last rows come out as they do on their own."""
+    from batchgen_amd.attention.gated_residual_norm import gated_residual_rmsnorm, gated_residual_rmsnorm_int8_quant
+    from batchgen_amd.moe.token_sort import sort_tokens, token_sort_plan, unsort_tokens
+    from batchgen_amd.quantization.int8 import int8_linear, int8_quant_rows
+    n, k, h, e = 40000, 8, 8192, 64
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.randn(n, h, device=dev, generator=g, dtype=torch.bfloat16).requires_grad_(True)
+    ids = torch.rand(n, e, device=dev, generator=g).topk(k, 1).indices
+    plan = token_sort_plan(ids, e)
+    rows = sort_tokens(x, plan)
+    assert rows.numel() * 2 > 1 << 32
+    back = unsort_tokens(rows, plan)
+    assert torch.equal(back, 8 * x.detach())              # eight equal terms: exact
+    (dx,) = torch.autograd.grad(back, x, torch.ones_like(back))
+    assert bool((dx == 8).all())
+    last = plan.topk_pos[-1].long()
+    assert torch.equal(rows.detach()[last], x.detach()[-1:].expand(k, h))
+    del rows, back, dx, x
+    torch.cuda.empty_cache()
+    m, kk, nn = 620000, 7168, 48
+    q = torch.randint(-127, 128, (m, kk), device=dev, generator=g, dtype=torch.int8)
+    w = torch.randint(-127, 128, (nn, kk), device=dev, generator=g, dtype=torch.int8)
+    s, ws = torch.rand(m, device=dev, generator=g), torch.rand(nn, device=dev, generator=g)
+    out = int8_linear(q, w, ws, x_scale=s)
+    assert torch.equal(out[-300:], int8_linear(q[-300:].clone(), w, ws, x_scale=s[-300:].clone()))
+    del q, out
+    torch.cuda.empty_cache()
+    r, hh = 300000, 8192
+    b, res = (torch.randn(r, hh, device=dev, generator=g, dtype=torch.bfloat16).requires_grad_(True) for _ in range(2))
+    pre = torch.rand(hh, device=dev, generator=g).to(torch.bfloat16)
+    y, nrm = gated_residual_rmsnorm(b, res, post_weight=pre, pre_weight=pre)
+    db, dr = torch.autograd.grad((y, nrm), (b, res), (y.detach(), nrm.detach()))
+    tail = [t.detach()[-5:].clone().requires_grad_(True) for t in (b, res)]
+    ty, tn = gated_residual_rmsnorm(*tail, post_weight=pre, pre_weight=pre)
+    tdb, tdr = torch.autograd.grad((ty, tn), tail, (ty.detach(), tn.detach()))
+    # another number of vectors per thread: another order of the row sums, at most a step of the output type away
+    for got, want in ((y[-5:], ty), (nrm[-5:], tn), (db[-5:], tdb), (dr[-5:], tdr)):
+        want = want.detach().to("cpu", ref.F64)
+        ref.assert_within(got, want, 2 * ref.half_step(torch.bfloat16, want) * (1 + 2 ** -7) + 2 ** -16 * want.abs().max(), "tail")
+    del y, nrm, db, dr
+    q, qs = int8_quant_rows(b.detach())
+    tq, tqs = int8_quant_rows(b.detach()[-5:].clone())
+    assert torch.equal(q[-5:], tq) and torch.equal(qs[-5:], tqs)
+    del q
+    with torch.no_grad():
+        q8 = gated_residual_rmsnorm_int8_quant(b, res, post_weight=pre, pre_weight=pre)
+        tq = int8_quant_rows(q8[1][-5:].clone())
+        assert torch.equal(q8[2][-5:], tq[0]) and torch.equal(q8[3][-5:], tq[1])
