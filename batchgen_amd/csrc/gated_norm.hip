@@ -184,7 +184,7 @@ __global__ __launch_bounds__(1024) void gated_norm_kernel(NormArgs a) {
 }
 
 // Rows are walked by gridDim.x blocks; the next row's operands are requested, still packed, before this row's exchange of
-// sums, so that a CU always has a row (57 KB at h = 7168) on its way while its VALU (about 45 operations per element)
+// sums, so that a CU always has a row (57 KB at h = 7168) on its way while its VALU (about 40 operations per element)
 // works on another.  What the blocks sum over their rows lives in LDS, eight floats per thread and kind (in registers it
 // takes the place of that next row, or of a second block per CU).  Order of the planes: post, pre, gate.
 // ACC_LDS = false (rows wider than LDS holds, h > 8192): accumulators in registers.
@@ -266,17 +266,16 @@ __global__ __launch_bounds__(1024) void gated_norm_backward_kernel(NormArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         bh[u][i] *= i1;
-        const float y = __builtin_fmaf(token * sg[u][i], bh[u][i] * w1[u][i], yh[u][i]);
-        yh[u][i] = norm && i < left ? y * i2 : 0.0f;
-        if (norm) {
+        const float cb = sg[u][i] * (w1[u][i] * bh[u][i]);
+        if (norm) {                                        // (past the row's end every operand is 0, and so is yh)
+          yh[u][i] = __builtin_fmaf(token, cb, yh[u][i]) * i2;
           const float t = dn[i] * w2[i];
           sum[0] = __builtin_fmaf(t, yh[u][i], sum[0]);
           e[u][i] = __builtin_fmaf(i2, t, e[u][i]);
           dw2[i] = dn[i] * yh[u][i];
+          sum[2] = __builtin_fmaf(cb, yh[u][i], sum[2]);
         }
-        const float cb = sg[u][i] * w1[u][i] * bh[u][i];
         sum[1] = __builtin_fmaf(cb, e[u][i], sum[1]);
-        sum[2] = __builtin_fmaf(cb, yh[u][i], sum[2]);
       }
       if (norm && a.want_pre) add(1, u, dw2);
     }
@@ -293,13 +292,16 @@ __global__ __launch_bounds__(1024) void gated_norm_backward_kernel(NormArgs a) {
     for (int u = 0; u < V; ++u) {
       const int c = threadIdx.x * 8 + u * step, left = a.h - c;
       float db[8], dw1[8], gd[8];
+      if (a.gate_mode == BGMOE_GATE_TOKEN)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sg[u][i] *= token;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        e[u][i] = __builtin_fmaf(-m, yh[u][i], e[u][i]);   // Dy
-        const float dp = token * sg[u][i] * e[u][i];
+        if (norm) e[u][i] = __builtin_fmaf(-m, yh[u][i], e[u][i]);   // Dy
+        const float dp = sg[u][i] * e[u][i];
         dw1[i] = dp * bh[u][i];
-        gd[i] = a.scale * e[u][i] * bh[u][i] * w1[u][i];
-        db[i] = a.post ? i1 * (dp * w1[u][i] - bh[u][i] * mb) : dp;
+        gd[i] = a.scale * e[u][i] * (bh[u][i] * w1[u][i]);
+        db[i] = a.post ? i1 * __builtin_fmaf(-mb, bh[u][i], dp * w1[u][i]) : dp;
       }
       if (a.d_block) store8<T, NT>(a.d_block, base + c, left, db);
       if (a.d_residual) store8<T, NT>(a.d_residual, base + c, left, e[u]);
@@ -365,14 +367,14 @@ int forward_vecs(int64_t rows, int h) { return h > 8192 || rows >= 1024 ? 2 : 1;
 int backward_vecs(int h) { return h > 8192 ? 2 : 1; }
 // Blocks of the gradient pass: what is resident at 128 registers per thread (1024 threads per CU), at most one per row.
 // Fewer blocks would write fewer planes, but a row takes a block about 2.2 us: 1024 x 7168 35 us with 256 blocks, 82
-// with 64; 4096 x 2048 56 us with 256.  16384 x 7168 bf16: 356 us, 4.0 TB/s.
+// with 64; 4096 x 2048 56 us with 256.  16384 x 7168 bf16: 337 us, 4.2 TB/s.
 int64_t backward_blocks(int64_t rows, int h) {
   const int64_t blocks = 256 * (1024 / threads_for(h, backward_vecs(h)));
   return rows < blocks ? rows : blocks;
 }
 
 // Whether a pass over `operands` row matrices moves more than the last-level cache holds, which it then bypasses: forward
-// of 16384 x 7168 bf16 230 -> 168 us (5.6 TB/s), with the int8 form 269 -> 203, gradient 361 -> 356; gradient of 16384 x
+// of 16384 x 7168 bf16 230 -> 168 us (5.6 TB/s), with the int8 form 269 -> 203; gradient of 16384 x
 // 2048 116 -> 96 us.  4096 x 7168, which fits, 45.2 us through it and 47.5 past it.
 template <typename T>
 bool past_cache(const NormArgs& a, int operands) { return a.rows * a.h * T::kBytes * operands > (256LL << 20); }
