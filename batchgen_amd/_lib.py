@@ -111,8 +111,7 @@ _SIGS = {
     "bgmoe_fp8_fused_s1_balanced": (i32, [C.POINTER(Fp8Act), C.POINTER(Fp8Weight), C.POINTER(Fp8Weight), vp, vp, i32,
                                           i64, i32, i32, vp, vp, vp, i64, i64, i64, vp, sz, vp]),
     "bgmoe_int8_quant_rows": (i32, [vp, i32, i64, i64, i32, vp, vp, vp]),
-    "bgmoe_int8_gemm_workspace_bytes": (sz, [i64, i32, i32]),
-    "bgmoe_int8_gemm": (i32, [vp, i64, vp, vp, vp, vp, i64, i32, i32, vp, i32, i64, vp, sz, vp]),
+    "bgmoe_int8_gemm": (i32, [vp, i64, vp, vp, vp, vp, i64, i32, i32, vp, i32, i64, vp]),
     "bgmoe_int8_linear_workspace_bytes": (sz, [i64, i32, i32]),
     "bgmoe_int8_linear": (i32, [vp, i32, i64, vp, vp, vp, i64, i32, i32, vp, i32, i64, vp, sz, vp]),
     "bgmoe_int8_grouped_gemm": (i32, [vp, vp, vp, i64, vp, i64, vp, vp, i32, i64, i32, i32, vp, i32, vp]),

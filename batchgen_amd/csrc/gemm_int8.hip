@@ -870,14 +870,9 @@ extern "C" int bgmoe_int8_quant_rows(const void* x, int dtype, int64_t x_row_str
 #undef BGMOE_CALL
 }
 
-extern "C" size_t bgmoe_int8_gemm_workspace_bytes(int64_t m, int n, int k) {
-  (void)m; (void)n; (void)k;
-  return 0;
-}
-
 extern "C" int bgmoe_int8_gemm(const int8_t* x, int64_t x_row_stride, const float* x_scale, const int8_t* w,
                                const float* w_scale, const float* bias, int64_t m, int n, int k, void* out, int out_dtype,
-                               int64_t out_row_stride, void* workspace, size_t workspace_bytes, bgmoe_stream_t stream) {
+                               int64_t out_row_stride, bgmoe_stream_t stream) {
   int rc = check_sizes("int8_gemm", m, n, k, out_dtype);
   if (rc != BGMOE_OK) return rc;
   if (m == 0 || n == 0) return BGMOE_OK;
@@ -887,7 +882,6 @@ extern "C" int bgmoe_int8_gemm(const int8_t* x, int64_t x_row_stride, const floa
   BGMOE_REQUIRE(x_row_stride >= k && x_row_stride < (1LL << 24), "int8_gemm: x_row_stride %lld outside [k, 2^24)",
                 (long long)x_row_stride);
   BGMOE_REQUIRE(out_row_stride >= n, "int8_gemm: out_row_stride %lld is smaller than n=%d", (long long)out_row_stride, n);
-  (void)workspace; (void)workspace_bytes;
   rc = ensure_init();
   if (rc != BGMOE_OK) return rc;
   Int8Args a{};
@@ -901,7 +895,7 @@ static size_t linear_scale_bytes(int64_t m) { return ((size_t)m * 4 + 15) / 16 *
 
 extern "C" size_t bgmoe_int8_linear_workspace_bytes(int64_t m, int n, int k) {
   if (m <= 0 || n <= 0 || k <= 0) return 0;
-  return linear_rows_bytes(m, k) + linear_scale_bytes(m) + bgmoe_int8_gemm_workspace_bytes(m, n, k);
+  return linear_rows_bytes(m, k) + linear_scale_bytes(m);
 }
 
 extern "C" int bgmoe_int8_linear(const void* x, int x_dtype, int64_t x_row_stride, const int8_t* w, const float* w_scale,
@@ -920,11 +914,10 @@ extern "C" int bgmoe_int8_linear(const void* x, int x_dtype, int64_t x_row_strid
   uint8_t* ws = (uint8_t*)workspace;
   int8_t* q = (int8_t*)ws;
   float* qs = (float*)(ws + linear_rows_bytes(m, k));
-  uint8_t* rest = ws + linear_rows_bytes(m, k) + linear_scale_bytes(m);
   rc = bgmoe_int8_quant_rows(x, x_dtype, x_row_stride, m, k, q, qs, stream);
   if (rc != BGMOE_OK) return rc;
-  return bgmoe_int8_gemm(q, k, qs, w, w_scale, bias, m, n, k, out, out_dtype, out_row_stride, rest,
-                         workspace_bytes - (size_t)(rest - ws), stream);
+  return bgmoe_int8_gemm(q, k, qs, w, w_scale, bias, m, n, k, out, out_dtype, out_row_stride,
+                         stream);
 }
 
 static int grouped(const char* what, Int8Args& a, int groups, int out_dtype, bgmoe_stream_t stream) {

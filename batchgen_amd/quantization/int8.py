@@ -96,20 +96,16 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     if m == 0 or n == 0:
         return out
     if quantised:
-        if x2.data_ptr() % 16 or x2.stride(0) % 16:
-            x2 = x2.contiguous() if x2.stride(0) % 16 else x2.clone()
-        ws = _workspace(lib().bgmoe_int8_gemm_workspace_bytes(m, n, k), x.device)
-        ck.launch(x.device, lib().bgmoe_int8_gemm, ptr(x2), x2.stride(0) if m > 1 else k, ptr(x_scale), ptr(weight),
-                  ptr(weight_scale), ptr(bias), m, n, k, ptr(out), code, n, ptr(ws), 0 if ws is None else ws.numel())
+        row_stride = x2.stride(0) if m > 1 else k
+        if x2.data_ptr() % 16 or row_stride % 16 or row_stride >= 1 << 24:  # what the kernels' loads take
+            x2, row_stride = x2.clone(memory_format=torch.contiguous_format), k
+        ck.launch(x.device, lib().bgmoe_int8_gemm, ptr(x2), row_stride, ptr(x_scale), ptr(weight),
+                  ptr(weight_scale), ptr(bias), m, n, k, ptr(out), code, n)
     else:
         x_code = ck.dtype_code(x, "x")
-        ws = _workspace(lib().bgmoe_int8_linear_workspace_bytes(m, n, k), x.device)
+        # scratch of one call from torch's allocator: it follows the stream it is used on, and under graph capture it
+        # belongs to the graph, so two captured graphs never share it
+        ws = torch.empty(lib().bgmoe_int8_linear_workspace_bytes(m, n, k), dtype=torch.uint8, device=x.device)
         ck.launch(x.device, lib().bgmoe_int8_linear, ptr(x2), x_code, x2.stride(0), ptr(weight), ptr(weight_scale),
                   ptr(bias), m, n, k, ptr(out), code, n, ptr(ws), ws.numel())
     return out
-
-
-def _workspace(nbytes: int, device):
-    """Scratch of one call, from torch's allocator: it follows the stream it is used on, and under graph capture it
-    belongs to the graph, so two captured graphs never share it."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None

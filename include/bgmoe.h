@@ -812,12 +812,10 @@ int bgmoe_int8_quant_rows(const void* x, int dtype, int64_t x_row_stride, int64_
 /* out[t][j] = (sum_k x[t][k] * w[j][k]) * x_scale[t] * w_scale[j] (+ bias[j]): the sum is exact (int32 MFMA
  * accumulators; k <= 131071), the two scalings and the bias are fp32, one rounding to out_dtype.  x [m,k] int8 with
  * x_row_stride bytes between rows, w [n,k] int8 contiguous; k % 16 == 0, both 16-byte aligned, x_row_stride % 16 == 0.
- * out rows are out_row_stride elements apart.  workspace: bgmoe_int8_gemm_workspace_bytes(m,n,k) bytes (0 = none
- * needed): the int32 planes of a K split when m is small.  Results do not depend on the split. */
-size_t bgmoe_int8_gemm_workspace_bytes(int64_t m, int n, int k);
+ * out rows are out_row_stride elements apart.  Results do not depend on how K is split; no workspace is needed. */
 int bgmoe_int8_gemm(const int8_t* x, int64_t x_row_stride, const float* x_scale, const int8_t* w, const float* w_scale,
                     const float* bias, int64_t m, int n, int k, void* out, int out_dtype, int64_t out_row_stride,
-                    void* workspace, size_t workspace_bytes, bgmoe_stream_t stream);
+                    bgmoe_stream_t stream);
 
 /* bgmoe_int8_quant_rows followed by bgmoe_int8_gemm in one call, with the same bits; the int8 rows and their scales
  * live in the workspace (bgmoe_int8_linear_workspace_bytes(m,n,k) bytes, 16-byte aligned). */

@@ -111,7 +111,7 @@ def test_int8_refusals():
     f = "bgmoe_int8_gemm"
 
     def args(**kw):
-        a = dict(x=P, ldx=64, xs=P, w=P, ws=P, bias=None, m=4, n=8, k=64, out=P, dt=0, ldo=8, work=None, nbytes=0, st=None)
+        a = dict(x=P, ldx=64, xs=P, w=P, ws=P, bias=None, m=4, n=8, k=64, out=P, dt=0, ldo=8, st=None)
         a.update(kw)
         return tuple(a.values())
     refused(f, *args(k=40), says="multiple of 16")
@@ -146,13 +146,10 @@ def test_int8_rings_wait_for_what_they_read(mode, schedule, m, n, k):
     x, w = (emu.guarded(rng.integers(-128, 128, s, dtype=np.int8)) for s in ((m, k), (n, k)))
     xs, ws = (emu.guarded(rng.uniform(0.5, 1.5, s).astype(np.float32)) for s in (m, n))
     out = emu.guarded(np.zeros((m, n), np.float32))
-    need = h.bgmoe_int8_gemm_workspace_bytes(m, n, k)
-    work = emu.guarded(np.full(max(need, 1), 255, np.uint8))
     h.emu_set_async_mode(mode)
     h.emu_set_schedule(schedule)
     try:
-        emu.ok(h, h.bgmoe_int8_gemm(emu.p(x), k, emu.p(xs), emu.p(w), emu.p(ws), None, m, n, k, emu.p(out), 2, n, emu.p(work),
-                                    need, None))
+        emu.ok(h, h.bgmoe_int8_gemm(emu.p(x), k, emu.p(xs), emu.p(w), emu.p(ws), None, m, n, k, emu.p(out), 2, n, None))
     finally:
         h.emu_set_async_mode(0)
         h.emu_set_schedule(0)

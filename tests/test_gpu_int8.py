@@ -98,6 +98,19 @@ def test_dense_product(dev, shape):
         check_product(got, want, b, f"int8_linear {shape} {dtype}")
 
 
+# rows, elements between them, element the first starts at
+@pytest.mark.parametrize("view", [(3, 64, 5), (1, 71, 3), (3, 72, 0), (3, 80, 16), (40, 70, 1), (2, 1 << 24, 0)], ids=str)
+def test_rows_at_any_address_and_stride(dev, view):
+    from batchgen_amd.quantization.int8 import int8_linear
+    m, stride, first = view
+    base = ints(50, (m - 1) * stride + 64 + first).to(dev)
+    x = base.as_strided((m, 64), (stride, 1), first)
+    w, xs, ws = ints(51, 33, 64).to(dev), scales(52, m).to(dev), scales(53, 33).to(dev)
+    check_product(int8_linear(x, w, ws, x_scale=xs), product(*(t.cpu() for t in (x, xs, w, ws))), None, f"view {view}")
+    xb = torch.randn(base.shape, generator=torch.Generator().manual_seed(54)).to(dev, torch.bfloat16).as_strided((m, 64), (stride, 1), first)
+    assert torch.equal(int8_linear(xb, w, ws), int8_linear(xb.cpu().contiguous().to(dev), w, ws))
+
+
 @pytest.mark.parametrize("shape", [(1, 200, 4096), (5, 64, 20000), (2, 100, 16400), (100, 70, 7168)], ids=str)
 def test_dense_product_long_k(dev, shape):
     from batchgen_amd.quantization.int8 import int8_linear
