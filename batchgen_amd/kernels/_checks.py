@@ -90,6 +90,13 @@ def dtype_code(t: torch.Tensor, name: str) -> int:
     return code
 
 
+def int32(value: int, name: str) -> int:
+    """``value`` where the C ABI takes an ``int``: ctypes would cut a larger one without a word."""
+    if not -0x80000000 <= value <= 0x7fffffff:
+        fail(f"{name} = {value} does not fit 32 bits")
+    return value
+
+
 def rows_of(t: torch.Tensor, name: str) -> torch.Tensor:
     """``t [..., K]`` as ``[rows, K]`` whose rows are contiguous (a 2-D tensor may keep a stride between its rows)."""
     if t.dim() == 2 and t.is_contiguous():

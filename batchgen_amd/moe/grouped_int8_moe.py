@@ -24,6 +24,8 @@ def _rows(x, x_scale, seqlens, cu_seqlens, e):
     if x.dim() != 2:
         ck.fail(f"x must be int8 [rows, K], got {tuple(x.shape)}")
     m, k = x.shape
+    ck.int32(k, "K")
+    ck.int32(e, "E")
     ck.cuda_tensor(x, x_scale, torch.float32, "x_scale")
     if x_scale.numel() != m:
         ck.fail(f"x_scale must hold one element per row ({m}), got {x_scale.numel()}")
@@ -53,6 +55,7 @@ def _weight(x, w, s, k, name):
 
 
 def _out(x, out, out_dtype, m, n):
+    ck.int32(n, "N")
     dt = out.dtype if out is not None else (out_dtype or torch.bfloat16)
     code = ck.DTYPE_CODE.get(dt)
     if code is None or (out is not None and out_dtype not in (None, out.dtype)):

@@ -53,7 +53,9 @@ def token_sort_plan(topk_ids: torch.Tensor, num_experts: int, expert_start: int 
     if topk_ids.dim() != 2 or not 1 <= topk_ids.size(1) <= MAX_TOP_K:
         ck.fail(f"topk_ids must be [N, K] with K in [1, {MAX_TOP_K}], got {tuple(topk_ids.shape)}")
     n, k = topk_ids.shape
-    e, row_align = int(num_experts), int(row_align)
+    e, row_align = ck.int32(int(num_experts), "num_experts"), ck.int32(int(row_align), "row_align")
+    ck.int32(n * k, "N*K")
+    ck.int32(int(expert_start), "expert_start")
     if row_align <= 0 or row_align & (row_align - 1):
         ck.fail(f"row_align must be a positive power of two, got {row_align}")
     ids = topk_ids.contiguous()
@@ -73,6 +75,7 @@ def _tokens(x, plan, name, rows):
     ck.same_device(plan.topk_pos, x, name)
     if x.dim() != 2 or x.size(0) != rows:
         ck.fail(f"{name} must be [{rows}, H], got {tuple(x.shape)}")
+    ck.int32(x.size(1), "H")
     return ck.rows_of(x, name)
 
 

@@ -30,6 +30,8 @@ def int8_quant_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
     ck.gpu(x, "x")
     no_grad_needed("int8_quant_rows", x)
     code = ck.dtype_code(x, "x")
+    if x.dim():
+        ck.int32(x.size(-1), "K")
     x2 = ck.rows_of(x, "x")
     rows, k = x2.shape
     if out is None:
@@ -66,6 +68,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     if weight.dim() != 2 or x.dim() < 1 or x.size(-1) != weight.size(1):
         ck.fail(f"int8_linear: x [..., K] and weight [N, K] do not fit: {tuple(x.shape)}, {tuple(weight.shape)}")
     n, k = weight.shape
+    ck.int32(n, "N")
+    ck.int32(k, "K")
     ck.cuda_tensor(x, weight_scale, torch.float32, "weight_scale")
     if weight_scale.numel() != n:
         ck.fail(f"weight_scale must hold N = {n} elements, got {weight_scale.numel()}")

@@ -77,6 +77,22 @@ def test_gradients(dev, shape, dtype, param, gate):
     check_grads(dev, ops, dtype, 0.7, dy, dn)
 
 
+@pytest.mark.parametrize("gate", GATES)
+@pytest.mark.parametrize("only", range(5))
+def test_gradient_of_one_leaf_alone(dev, only, gate):
+    ops = operands(37, 264, torch.bfloat16, gate)
+    if ops[only] is not None:
+        dy, dn = rand(27, 37, 264, dtype=torch.bfloat16), rand(28, 37, 264, dtype=torch.bfloat16)
+        check_grads(dev, ops, torch.bfloat16, 0.7, None if only == 4 else dy, dn, only)   # pre_weight acts on normed alone
+
+
+# the widest rows, and several rows per block at a width between the two register layouts' limits
+@pytest.mark.parametrize("shape,dtype,gate", [((5, 16384), torch.bfloat16, "channel"), ((3, 16384), torch.float32, "full"),
+                                              ((700, 7168), torch.bfloat16, "channel"), ((515, 8192), torch.float16, "token")], ids=str)
+def test_gradients_of_wide_rows(dev, shape, dtype, gate):
+    check_grads(dev, operands(*shape, dtype, gate), dtype, 0.7, rand(25, *shape, dtype=dtype), rand(26, *shape, dtype=dtype))
+
+
 @pytest.mark.parametrize("which", ["dy only", "dn only", "no post", "no pre", "neither norm"])
 def test_gradients_of_partial_calls(dev, which):
     ops = list(operands(9, 130, torch.float32, "token"))
@@ -92,16 +108,16 @@ def test_gradients_of_partial_calls(dev, which):
     check_grads(dev, ops, torch.float32, -0.3, dy, dn)
 
 
-def check_grads(dev, ops, dtype, scale, dy, dn):
-    leaves = [None if t is None else t.clone().to(dev).requires_grad_(True) for t in ops]
+def check_grads(dev, ops, dtype, scale, dy, dn, only=None):
+    leaves = [None if t is None else t.clone().to(dev).requires_grad_(only in (None, i)) for i, t in enumerate(ops)]
     block, residual, post, gate, pre = leaves
     y, n = api().gated_residual_rmsnorm(block, residual, post_weight=post, gate=gate, residual_scale=scale, pre_weight=pre,
                                         eps=EPS)
     outs = [(o, g.to(dev)) for o, g in ((y, dy), (n, dn)) if g is not None]
-    wanted = [t for t in leaves if t is not None]
+    wanted = [t for t in leaves if t is not None and t.requires_grad]
     grads = torch.autograd.grad([o for o, _ in outs], wanted, [g for _, g in outs], allow_unused=False)
     want, mag = ref.norm_grads(*ops[:4], scale, ops[4], EPS, dy, dn)
-    names = [m for m, t in zip(("block", "residual", "post", "gate", "pre"), leaves) if t is not None]
+    names = [m for m, t in zip(("block", "residual", "post", "gate", "pre"), leaves) if t is not None and t.requires_grad]
     c = ref.grad_roundings(ops[0].size(0))
     for name, leaf, got in zip(names, wanted, grads):
         assert got.dtype == leaf.dtype and got.shape == leaf.shape

@@ -303,6 +303,14 @@ def test_refusals(dev):
                                     ws[:1])):
         with pytest.raises(RuntimeError):
             bad()
+    wide = (1 << 32) + 64                                 # its low 32 bits are a valid K
+    for bad in (lambda: int8_quant_rows(x[0, 0].expand(1, wide)),
+                lambda: int8_linear(q[0, 0].expand(1, wide), torch.empty(0, wide, dtype=torch.int8, device=dev), ws[:0], x_scale=s[:1]),
+                lambda: int8_grouped_gemm(torch.empty(0, wide, dtype=torch.int8, device=dev), s[:0],
+                                          torch.empty(1, 0, wide, dtype=torch.int8, device=dev), ws[:0].view(1, 0),
+                                          torch.zeros(1, dtype=torch.int32, device=dev), torch.zeros(2, dtype=torch.int32, device=dev))):
+        with pytest.raises(RuntimeError):
+            bad()
     we, wse = w.view(1, 32, 64), ws.view(1, 32)
     n1 = torch.tensor([4], dtype=torch.int32, device=dev)
     cu = torch.tensor([0, 4], dtype=torch.int32, device=dev)

@@ -275,7 +275,11 @@ def test_refusals(dev):
                 lambda: t.token_sort_plan(torch.zeros(2, 33, dtype=torch.int32, device=dev), 4),
                 lambda: t.token_sort_plan(ids, 0), lambda: t.token_sort_plan(ids, 1025),
                 lambda: t.token_sort_plan(ids, 4, row_align=3), lambda: t.token_sort_plan(ids, 4, row_align=0),
-                lambda: t.token_sort_plan(ids, 4, expert_start=-1)):
+                lambda: t.token_sort_plan(ids, 4, expert_start=-1),
+                # sizes whose low 32 bits are valid
+                lambda: t.token_sort_plan(ids[:1, :1].expand((1 << 32) + 4, 1), 4), lambda: t.token_sort_plan(ids, (1 << 32) + 4),
+                lambda: t.token_sort_plan(ids, 4, expert_start=1 << 32), lambda: t.token_sort_plan(ids, 4, row_align=1 << 32),
+                lambda: t.sort_tokens(torch.zeros(1, 1, device=dev).expand(4, (1 << 32) + 4), t.token_sort_plan(ids, 4))):
         with pytest.raises(RuntimeError):
             bad()
     plan = t.token_sort_plan(ids, 4)
