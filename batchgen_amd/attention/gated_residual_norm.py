@@ -13,10 +13,10 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .._lib import lib, ptr
 from ..kernels import _checks as ck
+from ..kernels._autograd import no_second_gradient
 from ..quantization.int8 import no_grad_needed
 
 MAX_HIDDEN = 16384
@@ -98,9 +98,15 @@ def _backward(ctx, d_y, d_normed):
     return (*grads, None)
 
 
-# The gradient has none of its own.  once_differentiable says so where it matters, but costs 75 us a call: it wraps it
-# only while a graph of the backward pass is being recorded.
-_backward_once = once_differentiable(_backward)
+def _tied_to_sources(ctx, d_y, d_normed, grads):
+    """The gradients of (block, residual, post, gate, pre) with what each of them depends on."""
+    block, residual, post, gate, pre, _ = ctx.saved_tensors
+    if d_normed is not None:                              # through the second norm: on everything, but linearly on pre
+        every = (block, residual, post, gate, d_y, d_normed)
+        sources = ((*every, pre),) * 4 + (every,)
+    else:                                                 # y is linear in residual, post_weight and gate
+        sources = ((d_y, post, gate) + ((block,) if post is not None else ()), (d_y,), (d_y, block, gate), (d_y, block, post), ())
+    return [no_second_gradient("gated_residual_rmsnorm", g, *s) for g, s in zip(grads, sources)]
 
 
 class _GatedNorm(torch.autograd.Function):
@@ -118,7 +124,11 @@ class _GatedNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_y, d_normed):
-        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, d_y, d_normed)
+        if not torch.is_grad_enabled():
+            return _backward(ctx, d_y, d_normed)
+        with torch.no_grad():                             # a graph of the backward pass is being recorded
+            grads = _backward(ctx, d_y, d_normed)
+        return (*_tied_to_sources(ctx, d_y, d_normed, grads[:5]), None)
 
 
 def _contiguous(*tensors):

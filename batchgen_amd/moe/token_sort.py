@@ -17,10 +17,10 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .._lib import lib, ptr
 from ..kernels import _checks as ck
+from ..kernels._autograd import no_second_gradient
 from .dispatch_scatter_3d import ragged_row_capacity
 
 MAX_TOP_K = 32
@@ -106,10 +106,8 @@ def _run_unsort(rows, plan, weights, out):
     return out
 
 
-# The gradients have none of their own.  once_differentiable says so where it matters, but costs 75 us a call: it wraps
-# them only while a graph of the backward pass is being recorded.
 def _sort_backward(ctx, d_rows):
-    return _run_unsort(d_rows.contiguous(), ctx.plan, None, None), None
+    return _run_unsort(d_rows.contiguous(), ctx.plan, None, None)
 
 
 def _unsort_backward(ctx, d_out):
@@ -121,13 +119,10 @@ def _unsort_backward(ctx, d_out):
         ck.launch(rows.device, lib().bgmoe_token_unsort_backward, ptr(d_out), ptr(rows), ck.dtype_code(rows, "rows"),
                   ptr(plan.topk_pos), ptr(weights), plan.num_tokens, plan.top_k, rows.size(1), ptr(plan.meta),
                   ptr(plan.meta) + 4 * plan.num_experts, plan.num_experts, plan.capacity, ptr(d_rows), ptr(d_weights))
-    return d_rows, d_weights, None
+    return d_rows, d_weights
 
 
-_sort_backward_once = once_differentiable(_sort_backward)
-_unsort_backward_once = once_differentiable(_unsort_backward)
-
-
+# Grad mode is on in a backward pass only while a graph of it is being recorded (create_graph=True).
 class _Sort(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
@@ -136,7 +131,11 @@ class _Sort(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_rows):
-        return (_sort_backward_once if torch.is_grad_enabled() else _sort_backward)(ctx, d_rows)
+        if not torch.is_grad_enabled():
+            return _sort_backward(ctx, d_rows), None
+        with torch.no_grad():
+            d_x = _sort_backward(ctx, d_rows)
+        return no_second_gradient("sort_tokens", d_x, d_rows), None
 
 
 class _Unsort(torch.autograd.Function):
@@ -148,7 +147,13 @@ class _Unsort(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_out):
-        return (_unsort_backward_once if torch.is_grad_enabled() else _unsort_backward)(ctx, d_out)
+        if not torch.is_grad_enabled():
+            return (*_unsort_backward(ctx, d_out), None)
+        with torch.no_grad():
+            d_rows, d_weights = _unsort_backward(ctx, d_out)
+        rows, weights = ctx.saved_tensors
+        return (no_second_gradient("unsort_tokens", d_rows, d_out, weights),
+                no_second_gradient("unsort_tokens", d_weights, d_out, rows), None)
 
 
 def sort_tokens(x: torch.Tensor, plan: TokenSortPlan, out: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -1,0 +1,111 @@
+"""Ways of calling the token sort, the int8 products and the gated residual norm other than plainly with fresh operands."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def rand(seed, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def sort_api():
+    from batchgen_amd.moe import token_sort
+    return token_sort
+
+
+def norm_api():
+    from batchgen_amd.attention import gated_residual_norm
+    return gated_residual_norm
+
+
+def plan_for(dev, n=6, k=2, e=4, seed=1, **kw):
+    ids = torch.randint(0, e, (n, k), generator=torch.Generator().manual_seed(seed))
+    return sort_api().token_sort_plan(ids.to(dev), e, **kw)
+
+
+# ---- a gradient of a gradient ---------------------------------------------------------------------------------------
+NAMES = ("block", "residual", "post", "gate", "pre")
+
+
+def norm_leaves(dev, h=24, needed=NAMES, without=()):
+    ts = dict(block=rand(1, 4, h), residual=rand(2, 4, h), post=1 + 0.1 * rand(3, h), gate=torch.sigmoid(rand(4, h)),
+              pre=1 + 0.1 * rand(5, h))
+    return {m: None if m in without else t.to(dev).requires_grad_(m in needed) for m, t in ts.items()}
+
+
+def norm_of(v):
+    return norm_api().gated_residual_rmsnorm(v["block"], v["residual"], post_weight=v["post"], gate=v["gate"], pre_weight=v["pre"])
+
+
+@pytest.mark.parametrize("of", NAMES)
+@pytest.mark.parametrize("with_respect_to", NAMES)
+@pytest.mark.parametrize("through", ["y", "normed"])
+def test_norm_penalty_is_refused_with_a_constant_cotangent(dev, of, with_respect_to, through):
+    """d/d(with_respect_to) of |d out.sum() / d(of)|^2 + sum(with_respect_to): the first term's share may be left out only
+    where it is zero, by the same derivative of the plain formula in 64 bits."""
+    def plain(v):
+        i1 = torch.rsqrt(v["block"].square().mean(-1, keepdim=True) + 1e-5)
+        y = v["residual"] + v["gate"] * (v["block"] * i1 * v["post"])
+        return y, y * torch.rsqrt(y.square().mean(-1, keepdim=True) + 1e-5) * v["pre"]
+
+    def loss(v, f):
+        out = f(v)[0 if through == "y" else 1]
+        (g,) = torch.autograd.grad(out.sum(), v[of], create_graph=True, allow_unused=True)
+        return v[with_respect_to].sum() + (0 if g is None else g.square().sum())
+    v64 = {m: t.detach().cpu().double().requires_grad_(True) for m, t in norm_leaves("cpu").items()}
+    (want,) = torch.autograd.grad(loss(v64, plain), v64[with_respect_to])
+    depends = bool((want - 1).abs().max() > 1e-9)         # (a zero share is an exact zero but for rounding)
+    v = norm_leaves(dev)
+    total = loss(v, norm_of)
+    if depends:
+        with pytest.raises(RuntimeError, match="no gradient of its own"):
+            torch.autograd.grad(total, v[with_respect_to])
+    else:
+        (got,) = torch.autograd.grad(total, v[with_respect_to])
+        assert torch.equal(got, torch.ones_like(got))
+
+
+@pytest.mark.parametrize("without", [("post",), ("gate",), ("post", "gate")], ids=str)
+def test_norm_penalty_without_optional_operands(dev, without):
+    v = norm_leaves(dev, without=without)
+    y, n = norm_of(v)
+    (g,) = torch.autograd.grad(n.sum(), v["block"], create_graph=True)
+    with pytest.raises(RuntimeError, match="no gradient of its own"):
+        (g.square().sum() + v["block"].sum()).backward()
+    # y alone: linear in block without a norm behind it, and constant there if nothing else needs a gradient
+    v = norm_leaves(dev, needed=("block",), without=without)
+    (g,) = torch.autograd.grad(norm_of(v)[0].sum(), v["block"], create_graph=True)
+    assert g.requires_grad == ("post" not in without)
+
+
+def test_unsort_penalty_is_refused_with_a_constant_cotangent(dev):
+    t, plan = sort_api(), plan_for(dev)
+    rows, w = rand(7, plan.capacity, 8).to(dev).requires_grad_(True), rand(8, 6, 2).to(dev).requires_grad_(True)
+    g_rows, g_w = torch.autograd.grad(t.unsort_tokens(rows, plan, w).sum(), (rows, w), create_graph=True)
+    for g, leaf in ((g_rows, w), (g_w, rows)):            # d_rows depends on the weights, d_weights on the rows
+        with pytest.raises(RuntimeError, match="no gradient of its own"):
+            torch.autograd.grad(g.square().sum() + leaf.sum(), leaf, retain_graph=True)
+    # through the sort: a token's gradient depends on the weights too
+    x = rand(9, 6, 8).to(dev).requires_grad_(True)
+    (g,) = torch.autograd.grad(t.unsort_tokens(t.sort_tokens(x, plan), plan, w).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="no gradient of its own"):
+        torch.autograd.grad(g.square().sum() + w.sum(), w)
+
+
+def test_constant_first_gradients_stay_constants(dev):
+    """Linear operations: with a constant cotangent and constant other operands nothing is refused."""
+    t, plan = sort_api(), plan_for(dev)
+    x, w = rand(10, 6, 8).to(dev).requires_grad_(True), rand(11, 6, 2).to(dev)
+    rows = t.sort_tokens(x, plan)
+    for out in (rows, t.unsort_tokens(rows, plan), t.unsort_tokens(rows, plan, w)):
+        (g,) = torch.autograd.grad(out.sum(), x, create_graph=True)
+        (again,) = torch.autograd.grad(out.sum(), x, retain_graph=True)
+        assert not g.requires_grad and torch.equal(g, again)
+        (total,) = torch.autograd.grad(x.sum() + g.square().sum(), x)
+        assert torch.equal(total, torch.ones_like(total))
+    # a cotangent that needs a gradient: refused, as before
+    c = rand(12, plan.capacity, 8).to(dev).requires_grad_(True)
+    (g,) = torch.autograd.grad(t.sort_tokens(x, plan), x, c, create_graph=True)
+    with pytest.raises(RuntimeError, match="no gradient of its own"):
+        torch.autograd.grad(g.sum(), c)
