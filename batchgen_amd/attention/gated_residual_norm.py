@@ -141,8 +141,10 @@ def gated_residual_rmsnorm(block: torch.Tensor, residual: torch.Tensor, *, post_
                            ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``block``, ``residual`` ``[..., H]`` (bf16, fp16 or fp32, H <= 16384) -> ``(y, normed)``; ``normed`` is None
     without ``pre_weight``.  ``gate``: ``[H]`` (per channel), ``[..., 1]`` (per token) or ``[..., H]``.  Weights and gate
-    have block's type or fp32.  Gradients reach all five tensors, each in its tensor's type."""
+    have block's type or fp32.  Gradients reach all five tensors, each in its tensor's type; they have no gradient of their
+    own and there is no forward-mode derivative (asking for either raises)."""
     c = _Call(block, residual, post_weight, gate, pre_weight, residual_scale, eps)
+    ck.no_tangent("gated_residual_rmsnorm", block, residual, post_weight, gate, pre_weight)
     block, residual, post_weight, gate, pre_weight = _contiguous(block, residual, post_weight, gate, pre_weight)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                        for t in (block, residual, post_weight, gate, pre_weight)):

@@ -3,6 +3,7 @@ a violation raises RuntimeError before anything is launched)."""
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from .._lib import check
 
@@ -67,6 +68,17 @@ def combine_args(expert_output, topk_pos, topk_weights, output, n, h, k, out_dty
 
 
 FP8_BYTES = (torch.uint8, torch.float8_e4m3fn)
+
+
+def no_tangent(name: str, *tensors):
+    """Refuses tensors that carry a forward-mode tangent: the kernels see only the values, and a result without a
+    tangent would stand for a derivative of zero."""
+    if forward_ad._current_level < 0:                   # outside of torch.autograd.forward_ad.dual_level()
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            fail(f"{name} has no forward-mode derivative: its operands must not carry a tangent")
+
 
 def launch(device: torch.device, fn, *args):
     """``fn(*args, stream)`` with ``device`` current, on its current stream.  The context manager and the stream object of

@@ -9,6 +9,7 @@ fixed top-k, no gradient).  These are the same movement for training and for eve
     out = unsort_tokens(rows, plan, topk_weights)           # out[t] = sum_j w[t, j] * rows[topk_pos[t, j]]
 
 Gradients reach ``x``, ``rows`` and ``topk_weights``; no kernel uses atomics, so they are the same bits every time.
+They have no gradient of their own and there is no forward-mode derivative: asking for either raises.
 Ids outside ``[expert_start, expert_start + num_experts)`` (another rank's experts, ``-1`` on padding tokens) have no
 row: they add nothing to ``out`` and their weight gets gradient 0, whatever it holds.
 """
@@ -165,6 +166,7 @@ def sort_tokens(x: torch.Tensor, plan: TokenSortPlan, out: Optional[torch.Tensor
     x = _tokens(x, plan, "x", plan.num_tokens)
     if x.element_size() not in (1, 2, 4):
         ck.fail(f"x must have elements of 1, 2 or 4 bytes, got {x.dtype}")
+    ck.no_tangent("sort_tokens", x)
     wants_grad = torch.is_grad_enabled() and x.requires_grad
     if out is None:
         if wants_grad:
@@ -195,6 +197,7 @@ def unsort_tokens(rows: torch.Tensor, plan: TokenSortPlan, weights: Optional[tor
             weights = weights.float()
         if not weights.is_contiguous():
             weights = weights.contiguous()
+    ck.no_tangent("unsort_tokens", rows, weights)
     wants_grad = torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad))
     if out is None:
         if wants_grad:

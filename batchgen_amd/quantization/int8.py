@@ -4,7 +4,8 @@ The product over rows grouped by expert is ``batchgen_amd.moe.grouped_int8_moe``
 ``q[t, k] = rint(x[t, k] / s[t])`` with ``s[t] = max_k |x[t, k]| / 127``;
 ``out[t, j] = (sum_k q[t, k] * w[j, k]) * s[t] * c[j] (+ bias[j])``: the sum is an exact 32-bit integer, the rest fp32
 with one rounding to the output type.  A token that holds an infinity or a NaN gives NaN outputs.  Both ops belong to
-inference: they have no gradient and refuse operands that require one while grad mode is on.  They have no counterpart
+inference: they have no derivative and refuse operands that require a gradient while grad mode is on, or that carry
+a forward-mode tangent.  They have no counterpart
 in the reference, whose quantised products are FP8 and MXFP4.
 """
 from __future__ import annotations
@@ -18,6 +19,7 @@ from ..kernels import _checks as ck
 
 
 def no_grad_needed(name: str, *tensors):
+    ck.no_tangent(name, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:

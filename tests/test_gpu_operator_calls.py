@@ -109,3 +109,45 @@ def test_constant_first_gradients_stay_constants(dev):
     (g,) = torch.autograd.grad(t.sort_tokens(x, plan), x, c, create_graph=True)
     with pytest.raises(RuntimeError, match="no gradient of its own"):
         torch.autograd.grad(g.sum(), c)
+
+
+# ---- forward mode ---------------------------------------------------------------------------------------------------
+def calls_with_one_marked_operand(dev, mark):
+    """(name, call) for every public operation and floating operand of it; ``mark`` makes the operand what is tested."""
+    from batchgen_amd.moe.grouped_int8_moe import int8_fused_s1, int8_grouped_gemm
+    from batchgen_amd.quantization.int8 import int8_linear, int8_quant_rows
+    t, plan = sort_api(), plan_for(dev)
+    i8 = lambda *s: torch.ones(*s, dtype=torch.int8, device=dev)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)
+    norm = dict(block=rand(1, 4, 32), residual=rand(2, 4, 32), post_weight=rand(3, 32), gate=rand(4, 32), pre_weight=rand(5, 32))
+    ops = [
+        ("sort_tokens", lambda x: t.sort_tokens(x, plan), dict(x=rand(6, 6, 8))),
+        ("unsort_tokens", lambda rows, w: t.unsort_tokens(rows, plan, w), dict(rows=rand(7, plan.capacity, 8), w=rand(8, 6, 2))),
+        ("unsort_tokens, cast weights", lambda rows, w: t.unsort_tokens(rows, plan, w),
+         dict(rows=rand(7, plan.capacity, 8), w=rand(8, 6, 2).half())),
+        ("gated_residual_rmsnorm", norm_api().gated_residual_rmsnorm, norm),
+        ("gated_residual_rmsnorm_int8_quant", norm_api().gated_residual_rmsnorm_int8_quant, norm),
+        ("int8_quant_rows", int8_quant_rows, dict(x=rand(9, 4, 32))),
+        ("int8_linear", lambda x, ws, b: int8_linear(x, i8(8, 32), ws, bias=b), dict(x=rand(9, 4, 32), ws=rand(10, 8), b=rand(11, 8))),
+        ("int8_linear, int8 rows", lambda xs, ws: int8_linear(i8(4, 32), i8(8, 32), ws, x_scale=xs), dict(xs=rand(9, 4), ws=rand(10, 8))),
+        ("int8_grouped_gemm", lambda xs, ws: int8_grouped_gemm(i8(4, 32), xs, i8(1, 8, 32), ws, i32(4), i32(0, 4)),
+         dict(xs=rand(9, 4), ws=rand(10, 1, 8))),
+        ("int8_fused_s1", lambda xs, g, u: int8_fused_s1(i8(4, 32), xs, i8(1, 8, 32), g, i8(1, 8, 32), u, i32(4), i32(0, 4)),
+         dict(xs=rand(9, 4), g=rand(10, 1, 8), u=rand(11, 1, 8))),
+    ]
+    for name, f, operands in ops:
+        operands = {m: v.to(dev) for m, v in operands.items()}
+        for marked in operands:
+            yield f"{name}: {marked}", lambda f=f, o=operands, marked=marked: f(**{m: mark(v) if m == marked else v for m, v in o.items()})
+
+
+def test_operands_with_a_tangent_are_refused(dev):
+    from torch.autograd import forward_ad
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            for name, call in calls_with_one_marked_operand(dev, lambda v: forward_ad.make_dual(v, torch.ones_like(v))):
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call()
+                    pytest.fail(f"{name} dropped the tangent")
+            for name, call in calls_with_one_marked_operand(dev, lambda v: v):     # none carries one: they run
+                call()
