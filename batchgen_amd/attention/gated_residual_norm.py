@@ -170,10 +170,12 @@ def gated_residual_rmsnorm_int8_quant(block: torch.Tensor, residual: torch.Tenso
         ck.cuda_tensor(block, out, block.dtype, "out")
         if out.shape != block.shape:
             ck.fail(f"out must have the shape {tuple(block.shape)}, got {tuple(out.shape)}")
+        ck.writable("gated_residual_rmsnorm_int8_quant", out)
     block, residual, post_weight, gate, pre_weight = _contiguous(block, residual, post_weight, gate, pre_weight)
     y = torch.empty_like(block) if out is None else out
     normed = torch.empty_like(block)
     q = torch.empty(block.shape, dtype=torch.int8, device=c.device)
     scale = torch.empty(block.shape[:-1], dtype=torch.float32, device=c.device)
     _forward(c, block, residual, post_weight, gate, pre_weight, y, normed, q, scale, None, None)
+    ck.written(out)
     return y, normed, q, scale

@@ -80,6 +80,25 @@ def no_tangent(name: str, *tensors):
             fail(f"{name} has no forward-mode derivative: its operands must not carry a tangent")
 
 
+def writable(name: str, *outs):
+    """A caller's tensors that an op without a gradient is about to write: refused where autograd would go on with what
+    they were (they require a gradient in grad mode, or carry a forward-mode tangent)."""
+    no_tangent(name, *outs)
+    if torch.is_grad_enabled():
+        for t in outs:
+            if t is not None and t.requires_grad:
+                fail(f"{name} writes its output without a gradient: the tensor it writes must not require one in grad mode")
+
+
+def written(*outs):
+    """Tells autograd that these tensors have been written, as torch's own in-place operations do: the backward pass of
+    an earlier graph that saved one of them then raises instead of using the new values.  (Inference tensors have no
+    version and cannot be saved.)"""
+    for t in outs:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def launch(device: torch.device, fn, *args):
     """``fn(*args, stream)`` with ``device`` current, on its current stream.  The context manager and the stream object of
     torch.cuda take 4 us, as much as a short kernel; where the device is the current one already neither is needed."""

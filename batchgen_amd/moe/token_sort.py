@@ -176,7 +176,10 @@ def sort_tokens(x: torch.Tensor, plan: TokenSortPlan, out: Optional[torch.Tensor
         _buffer(out, x, (plan.capacity, x.size(1)), "out")
         if wants_grad:
             ck.fail("sort_tokens: out= has no gradient; call it without out, or under torch.no_grad()")
-    return _run_sort(x, plan, out)
+        ck.writable("sort_tokens", out)
+    rows = _run_sort(x, plan, out)
+    ck.written(out)
+    return rows
 
 
 def unsort_tokens(rows: torch.Tensor, plan: TokenSortPlan, weights: Optional[torch.Tensor] = None,
@@ -206,4 +209,7 @@ def unsort_tokens(rows: torch.Tensor, plan: TokenSortPlan, weights: Optional[tor
         _buffer(out, rows, (plan.num_tokens, rows.size(1)), "out")
         if wants_grad:
             ck.fail("unsort_tokens: out= has no gradient; call it without out, or under torch.no_grad()")
-    return _run_unsort(rows, plan, weights, out)
+        ck.writable("unsort_tokens", out)
+    tokens = _run_unsort(rows, plan, weights, out)
+    ck.written(out)
+    return tokens

@@ -31,6 +31,8 @@ def int8_quant_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
     """``x [..., K]`` (bf16, fp16 or fp32) -> ``(q int8 [..., K], scale fp32 [...])``."""
     ck.gpu(x, "x")
     no_grad_needed("int8_quant_rows", x)
+    held = (out, scale)                                   # the caller's tensors
+    ck.writable("int8_quant_rows", *held)
     code = ck.dtype_code(x, "x")
     if x.dim():
         ck.int32(x.size(-1), "K")
@@ -52,6 +54,7 @@ def int8_quant_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
         ck.fail("int8_quant_rows: rows without elements have no scale")
     if rows:
         ck.launch(x.device, lib().bgmoe_int8_quant_rows, ptr(x2), code, x2.stride(0), rows, k, ptr(out), ptr(scale))
+        ck.written(*held)
     return out, scale
 
 
@@ -66,6 +69,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     most 131071 (beyond it a sum could leave 32 bits)."""
     ck.gpu(x, "x")
     no_grad_needed("int8_linear", x, x_scale, weight_scale, bias)
+    held = out
+    ck.writable("int8_linear", held)
     ck.cuda_tensor(x, weight, torch.int8, "weight")
     if weight.dim() != 2 or x.dim() < 1 or x.size(-1) != weight.size(1):
         ck.fail(f"int8_linear: x [..., K] and weight [N, K] do not fit: {tuple(x.shape)}, {tuple(weight.shape)}")
@@ -114,4 +119,5 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         ws = torch.empty(lib().bgmoe_int8_linear_workspace_bytes(m, n, k), dtype=torch.uint8, device=x.device)
         ck.launch(x.device, lib().bgmoe_int8_linear, ptr(x2), x_code, x2.stride(0), ptr(weight), ptr(weight_scale),
                   ptr(bias), m, n, k, ptr(out), code, n, ptr(ws), ws.numel())
+    ck.written(held)
     return out

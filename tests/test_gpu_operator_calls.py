@@ -151,3 +151,74 @@ def test_operands_with_a_tangent_are_refused(dev):
                     pytest.fail(f"{name} dropped the tangent")
             for name, call in calls_with_one_marked_operand(dev, lambda v: v):     # none carries one: they run
                 call()
+
+
+# ---- a caller's output tensors --------------------------------------------------------------------------------------
+def calls_with_out(dev):
+    """(name, fresh tensors to write, call) for every public operation that writes a caller's tensors."""
+    from batchgen_amd.moe.grouped_int8_moe import int8_fused_s1, int8_grouped_gemm
+    from batchgen_amd.quantization.int8 import int8_linear, int8_quant_rows
+    t, plan = sort_api(), plan_for(dev)
+    i8 = lambda *s: torch.ones(*s, dtype=torch.int8, device=dev)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)
+    f = lambda seed, *s: rand(seed, *s).to(dev)
+    zeros = lambda *s: torch.zeros(*s, device=dev)
+    return [
+        ("sort_tokens", [zeros(plan.capacity, 8)], lambda o: t.sort_tokens(f(1, 6, 8), plan, out=o)),
+        ("unsort_tokens", [zeros(6, 8)], lambda o: t.unsort_tokens(f(1, plan.capacity, 8), plan, f(2, 6, 2), out=o)),
+        ("norm", [zeros(4, 32)], lambda o: norm_api().gated_residual_rmsnorm_int8_quant(f(1, 4, 32), f(2, 4, 32),
+                                                                                        pre_weight=f(3, 32), out=o)),
+        ("quantiser", [i8(4, 32), zeros(4)], lambda q, s: int8_quant_rows(f(1, 4, 32), out=q, scale=s)),
+        ("linear", [zeros(4, 8)], lambda o: int8_linear(f(1, 4, 32), i8(8, 32), f(2, 8), out=o)),
+        ("linear, int8 rows", [zeros(4, 8)], lambda o: int8_linear(i8(4, 32), i8(8, 32), f(2, 8), x_scale=f(3, 4), out=o)),
+        ("grouped", [zeros(4, 8)], lambda o: int8_grouped_gemm(i8(4, 32), f(1, 4), i8(1, 8, 32), f(2, 1, 8), i32(4), i32(0, 4), out=o)),
+        ("fused", [zeros(4, 8)], lambda o: int8_fused_s1(i8(4, 32), f(1, 4), i8(1, 8, 32), f(2, 1, 8), i8(1, 8, 32), f(3, 1, 8),
+                                                         i32(4), i32(0, 4), out=o)),
+    ]
+
+
+def test_an_earlier_graph_notices_that_its_tensor_was_overwritten(dev):
+    for name, outs, call in calls_with_out(dev):
+        for i, o in enumerate(outs):
+            if not o.is_floating_point():
+                continue
+            leaf = o.clone().requires_grad_(True)
+            held = leaf * 1.0                             # what an earlier graph saves
+            loss = held.square().sum()
+            with torch.no_grad():
+                call(*(held if j == i else p for j, p in enumerate(outs)))
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                loss.backward()
+                pytest.fail(f"{name}: the backward pass used the new values")
+
+
+def test_outputs_that_require_a_gradient_are_refused_in_grad_mode(dev):
+    from torch.autograd import forward_ad
+    for name, outs, call in calls_with_out(dev):
+        for i, o in enumerate(outs):
+            versions = [p._version for p in outs]
+            if o.is_floating_point():
+                with pytest.raises(RuntimeError, match="must not require"):
+                    call(*(p.clone().requires_grad_(True) if j == i else p for j, p in enumerate(outs)))
+                    pytest.fail(f"{name} took an output that requires a gradient")
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"), forward_ad.dual_level():
+                    call(*(forward_ad.make_dual(p, torch.ones_like(p)) if j == i else p for j, p in enumerate(outs)))
+            assert versions == [p._version for p in outs]                # refused: nothing written
+        with torch.no_grad():
+            call(*(p.clone().requires_grad_(p.is_floating_point()) for p in outs))
+        call(*outs)
+        assert all(p._version > 0 for p in outs), name
+
+
+def test_outputs_of_inference_mode(dev):
+    """Inference tensors have no version counter; ordinary ones are written in inference mode too."""
+    with torch.inference_mode():
+        cases = calls_with_out(dev)
+        for _, outs, call in cases:
+            call(*outs)
+    ordinary = calls_with_out(dev)
+    for (name, outs, call), (_, plain, same) in zip(cases, ordinary):
+        call(*outs)                                       # and outside of it, where no autograd can hold them
+        with torch.inference_mode():
+            same(*plain)
+        assert all(torch.equal(a, b) for a, b in zip(outs, plain)), name
