@@ -161,7 +161,8 @@ def gated_residual_rmsnorm_int8_quant(block: torch.Tensor, residual: torch.Tenso
                                       out: Optional[torch.Tensor] = None
                                       ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """The serving form: ``(y, normed, q, scale)`` with ``(q, scale)`` the bits of ``int8_quant_rows(normed)`` from the
-    same pass.  ``out`` takes ``y`` and may be ``residual`` itself (the running residual updated in place)."""
+    same pass.  ``out`` takes ``y`` and may be ``residual`` itself (the running residual updated in place), ``block`` or a
+    full ``gate``, but shares no part of their memory otherwise."""
     if pre_weight is None:
         ck.fail("gated_residual_rmsnorm_int8_quant needs pre_weight: the int8 rows are those of the second norm")
     no_grad_needed("gated_residual_rmsnorm_int8_quant", block, residual, post_weight, gate, pre_weight)
@@ -172,6 +173,8 @@ def gated_residual_rmsnorm_int8_quant(block: torch.Tensor, residual: torch.Tenso
             ck.fail(f"out must have the shape {tuple(block.shape)}, got {tuple(out.shape)}")
         ck.writable("gated_residual_rmsnorm_int8_quant", out)
     block, residual, post_weight, gate, pre_weight = _contiguous(block, residual, post_weight, gate, pre_weight)
+    if out is not None:                                   # a thread reads its elements of these before it writes y there
+        ck.apart("gated_residual_rmsnorm_int8_quant", out, post_weight, pre_weight, same_ok=(block, residual, gate))
     y = torch.empty_like(block) if out is None else out
     normed = torch.empty_like(block)
     q = torch.empty(block.shape, dtype=torch.int8, device=c.device)

@@ -90,6 +90,30 @@ def writable(name: str, *outs):
                 fail(f"{name} writes its output without a gradient: the tensor it writes must not require one in grad mode")
 
 
+def _end(t: torch.Tensor, start: int) -> int:
+    """The address behind the last element of ``t``."""
+    if t.is_contiguous():
+        return start + t.nbytes
+    return start + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else start
+
+
+def apart(name: str, out: torch.Tensor, *operands, same_ok=()):
+    """Refuses an output whose memory (first to last element) reaches into an operand's: blocks of one launch write the
+    one while others still read the other.  An operand of ``same_ok`` may be the output's memory as a whole."""
+    start = out.data_ptr()
+    end = start + out.nbytes                            # (outputs are contiguous)
+    for t in operands:
+        if t is not None:
+            p = t.data_ptr()
+            if p < end and _end(t, p) > start and p != 0:
+                fail(f"{name}: the output must not share memory with an operand")
+    for t in same_ok:
+        if t is not None:
+            p = t.data_ptr()
+            if p < end and _end(t, p) > start and p != 0 and not (p == start and t.is_contiguous() and t.nbytes == out.nbytes):
+                fail(f"{name}: the output must be an operand's whole memory or none of it")
+
+
 def written(*outs):
     """Tells autograd that these tensors have been written, as torch's own in-place operations do: the backward pass of
     an earlier graph that saved one of them then raises instead of using the new values.  (Inference tensors have no

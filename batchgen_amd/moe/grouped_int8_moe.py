@@ -73,7 +73,7 @@ def int8_grouped_gemm(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tens
                       out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``x`` int8 ``[rows, K]``, ``x_scale`` fp32 ``[rows]``, ``weight`` int8 ``[E, N, K]``, ``weight_scale`` fp32
     ``[E, N]``, ``seqlens`` int32 ``[E]``, ``cu_seqlens`` int32 ``[E (+ 1)]`` -> ``[rows, N]`` (bf16 unless ``out_dtype``
-    or ``out`` says otherwise; rows of no expert keep what ``out`` held)."""
+    or ``out`` says otherwise; rows of no expert keep what ``out`` held, which shares no memory with the operands)."""
     no_grad_needed("int8_grouped_gemm", x_scale, weight_scale)
     held = out
     ck.writable("int8_grouped_gemm", held)
@@ -83,6 +83,8 @@ def int8_grouped_gemm(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tens
     n = weight.size(1)
     out, code = _out(x, out, out_dtype, m, n)
     if m and n:
+        if held is not None:
+            ck.apart("int8_grouped_gemm", out, x, x_scale, weight, weight_scale, seqlens, cu_seqlens)
         ck.launch(x.device, lib().bgmoe_int8_grouped_gemm, ptr(x), ptr(x_scale), ptr(weight), weight.stride(0),
                   ptr(weight_scale), weight_scale.stride(0), ptr(seqlens), ptr(cu_seqlens), e, m, n, k, ptr(out),
                   code)
@@ -107,6 +109,8 @@ def int8_fused_s1(x: torch.Tensor, x_scale: torch.Tensor, gate_weight: torch.Ten
     n = gate_weight.size(1)
     out, code = _out(x, out, out_dtype, m, n)
     if m and n:
+        if held is not None:
+            ck.apart("int8_fused_s1", out, x, x_scale, gate_weight, gate_scale, up_weight, up_scale, seqlens, cu_seqlens)
         ck.launch(x.device, lib().bgmoe_int8_fused_s1, ptr(x), ptr(x_scale), ptr(gate_weight), gate_weight.stride(0),
                   ptr(gate_scale), gate_scale.stride(0), ptr(up_weight), up_weight.stride(0), ptr(up_scale),
                   up_scale.stride(0), ptr(seqlens), ptr(cu_seqlens), e, m, n, k, ptr(out), code)

@@ -162,7 +162,8 @@ def sort_tokens(x: torch.Tensor, plan: TokenSortPlan, out: Optional[torch.Tensor
     moves (int8 and FP8 rows, their fp32 scales as ``[N, 1]``); bf16, fp16 and fp32 have a gradient.
 
     Rows that hold no pair (alignment padding, rows at or past ``cu_seqlens[E]``) are zero in a fresh result; in a
-    caller's ``out`` they are left as they were.  ``out`` is for inference: it is refused where a gradient is wanted."""
+    caller's ``out`` they are left as they were.  ``out`` is for inference: it is refused where a gradient is wanted, and
+    shares no memory with ``x``."""
     x = _tokens(x, plan, "x", plan.num_tokens)
     if x.element_size() not in (1, 2, 4):
         ck.fail(f"x must have elements of 1, 2 or 4 bytes, got {x.dtype}")
@@ -177,6 +178,7 @@ def sort_tokens(x: torch.Tensor, plan: TokenSortPlan, out: Optional[torch.Tensor
         if wants_grad:
             ck.fail("sort_tokens: out= has no gradient; call it without out, or under torch.no_grad()")
         ck.writable("sort_tokens", out)
+        ck.apart("sort_tokens", out, x, plan.topk_pos, plan.meta)
     rows = _run_sort(x, plan, out)
     ck.written(out)
     return rows
@@ -186,7 +188,7 @@ def unsort_tokens(rows: torch.Tensor, plan: TokenSortPlan, weights: Optional[tor
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``rows [plan.capacity, H]`` (bf16, fp16 or fp32) -> ``[N, H]``: ``sum_j weights[t, j] * rows[topk_pos[t, j]]`` in
     fp32, one rounding; a token without a row gives zeros.  ``weights [N, K]`` (fp32, or a type that is cast to it);
-    None: a plain sum.  ``out`` is for inference."""
+    None: a plain sum.  ``out`` is for inference and shares no memory with the operands."""
     rows = _tokens(rows, plan, "rows", plan.capacity)
     if not rows.is_contiguous():
         rows = rows.contiguous()
@@ -210,6 +212,7 @@ def unsort_tokens(rows: torch.Tensor, plan: TokenSortPlan, weights: Optional[tor
         if wants_grad:
             ck.fail("unsort_tokens: out= has no gradient; call it without out, or under torch.no_grad()")
         ck.writable("unsort_tokens", out)
+        ck.apart("unsort_tokens", out, rows, weights, plan.topk_pos, plan.meta)
     tokens = _run_unsort(rows, plan, weights, out)
     ck.written(out)
     return tokens

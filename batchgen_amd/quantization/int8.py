@@ -28,7 +28,8 @@ def no_grad_needed(name: str, *tensors):
 
 def int8_quant_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
                     scale: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """``x [..., K]`` (bf16, fp16 or fp32) -> ``(q int8 [..., K], scale fp32 [...])``."""
+    """``x [..., K]`` (bf16, fp16 or fp32) -> ``(q int8 [..., K], scale fp32 [...])``; ``out`` / ``scale`` take them
+    and share no memory with ``x``."""
     ck.gpu(x, "x")
     no_grad_needed("int8_quant_rows", x)
     held = (out, scale)                                   # the caller's tensors
@@ -53,6 +54,10 @@ def int8_quant_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
     if rows and k == 0:
         ck.fail("int8_quant_rows: rows without elements have no scale")
     if rows:
+        if held[0] is not None:
+            ck.apart("int8_quant_rows", out, x2, scale)
+        if held[1] is not None:
+            ck.apart("int8_quant_rows", scale, x2, out)
         ck.launch(x.device, lib().bgmoe_int8_quant_rows, ptr(x2), code, x2.stride(0), rows, k, ptr(out), ptr(scale))
         ck.written(*held)
     return out, scale
@@ -65,7 +70,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
 
     ``x`` bf16, fp16 or fp32: quantised per token here (the bits of ``int8_quant_rows``), the output has its type unless
     ``out_dtype`` says otherwise.  ``x`` int8 with ``x_scale`` fp32 ``[...]``: used as it is, the output is bf16 unless
-    ``out_dtype`` says otherwise.  ``bias``: fp32 ``[N]``.  ``out``: contiguous ``[..., N]``.  K is a multiple of 16, at
+    ``out_dtype`` says otherwise.  ``bias``: fp32 ``[N]``.  ``out``: contiguous ``[..., N]``, apart from the
+    operands' memory (only an ``x`` that is quantised here may be ``out``).  K is a multiple of 16, at
     most 131071 (beyond it a sum could leave 32 bits)."""
     ck.gpu(x, "x")
     no_grad_needed("int8_linear", x, x_scale, weight_scale, bias)
@@ -110,10 +116,14 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         row_stride = x2.stride(0) if m > 1 else k
         if x2.data_ptr() % 16 or row_stride % 16 or row_stride >= 1 << 24:  # what the kernels' loads take
             x2, row_stride = x2.clone(memory_format=torch.contiguous_format), k
+        if held is not None:
+            ck.apart("int8_linear", out, x2, x_scale, weight, weight_scale, bias)
         ck.launch(x.device, lib().bgmoe_int8_gemm, ptr(x2), row_stride, ptr(x_scale), ptr(weight),
                   ptr(weight_scale), ptr(bias), m, n, k, ptr(out), code, n)
     else:
         x_code = ck.dtype_code(x, "x")
+        if held is not None:                              # (x itself is only read before the product: it may be out)
+            ck.apart("int8_linear", out, weight, weight_scale, bias)
         # scratch of one call from torch's allocator: it follows the stream it is used on, and under graph capture it
         # belongs to the graph, so two captured graphs never share it
         ws = torch.empty(lib().bgmoe_int8_linear_workspace_bytes(m, n, k), dtype=torch.uint8, device=x.device)

@@ -222,3 +222,66 @@ def test_outputs_of_inference_mode(dev):
         with torch.inference_mode():
             same(*plain)
         assert all(torch.equal(a, b) for a, b in zip(outs, plain)), name
+
+
+def test_outputs_that_share_memory_with_an_operand(dev):
+    from batchgen_amd.moe.grouped_int8_moe import int8_grouped_gemm
+    from batchgen_amd.quantization.int8 import int8_linear, int8_quant_rows
+    t, norm8 = sort_api(), norm_api().gated_residual_rmsnorm_int8_quant
+    plan = t.token_sort_plan((torch.arange(63, -1, -1) % 8).view(64, 1).to(dev), 8)       # as many rows as tokens
+    x = rand(1, 64, 16).to(dev)
+    w = rand(2, 64, 1).to(dev)
+    both = rand(3, 65 * 16).to(dev)
+    q = torch.ones(16, 16, dtype=torch.int8, device=dev)
+    ones = torch.ones(16, device=dev)
+    one = torch.tensor([16], dtype=torch.int32, device=dev)
+    seam = rand(4, 5, 32).to(dev)
+    pre = torch.ones(32, device=dev)
+    for bad in (lambda: t.sort_tokens(x, plan, out=x), lambda: t.unsort_tokens(x, plan, out=x),
+                lambda: t.sort_tokens(both[:1024].view(64, 16), plan, out=both[16:].view(64, 16)),
+                lambda: t.sort_tokens(both.as_strided((64, 4), (16, 1)), plan, out=both[:256].view(64, 4)),
+                lambda: t.unsort_tokens(both[16:].view(64, 16), plan, out=both[:1024].view(64, 16)),
+                lambda: t.unsort_tokens(rand(5, 64, 1).to(dev), plan, w, out=w),
+                lambda: t.unsort_tokens(rand(5, 64, 1).to(dev), plan, out=plan.topk_pos.view(torch.float32)),
+                lambda: norm8(seam[:4], seam[:4].clone(), pre_weight=pre, out=seam[1:]),
+                lambda: norm8(seam[:4].clone(), seam[1:], pre_weight=pre, out=seam[:4]),
+                lambda: norm8(seam[:1], seam[1:2], pre_weight=pre, out=pre.view(1, 32)),
+                lambda: int8_quant_rows(x, out=x.view(torch.int8)[:16].view(64, 16)),
+                lambda: int8_quant_rows(x, scale=x[:4].view(64)),
+                lambda: int8_quant_rows(x[:1, :4], out=ones[:1].view(torch.int8).view(1, 4), scale=ones[:1]),
+                lambda: int8_linear(x[:1], q, ones, out=ones.view(1, 16)),
+                lambda: int8_linear(x[:1], q, ones, bias=pre[:16], out=pre[:16].view(1, 16)),
+                lambda: int8_linear(both.view(torch.int8)[:256].view(16, 16), q, ones, x_scale=ones, out=both[:256].view(16, 16)),
+                lambda: int8_grouped_gemm(q, ones, q[:8].view(1, 8, 16), ones[:8].view(1, 8), one, one, out=q.view(torch.bfloat16).view(16, 8)),
+                lambda: int8_grouped_gemm(q, ones, q[:1].view(1, 1, 16), ones[:1].view(1, 1), one, one, out=ones.view(16, 1))):
+        before = [v.clone() for v in (x, w, both, q, ones, one, seam, pre, plan.topk_pos)]
+        with pytest.raises(RuntimeError, match="share memory|whole memory"):
+            bad()
+        for a, b in zip(before, (x, w, both, q, ones, one, seam, pre, plan.topk_pos)):
+            assert torch.equal(a, b)                      # refused before anything was written
+
+
+def test_outputs_that_may_be_an_operand(dev):
+    """The whole of block, residual or a full gate; the input of a product that is quantised first; memory beside an operand."""
+    from batchgen_amd.quantization.int8 import int8_linear
+    t, norm8 = sort_api(), norm_api().gated_residual_rmsnorm_int8_quant
+    block, residual, gate, pre = (rand(s, 4, 32).to(dev) for s in (1, 2, 3, 4))
+    want = norm8(block, residual, gate=gate, pre_weight=pre[0])
+    for i in range(3):
+        ops = [v.clone() for v in (block, residual, gate)]
+        got = norm8(*ops[:2], gate=ops[2], pre_weight=pre[0], out=ops[i])
+        assert got[0] is ops[i] and all(torch.equal(a, b) for a, b in zip(got, want)), i
+    # a residual that is copied because it is not contiguous does not share memory with the output any more
+    wide = torch.zeros(4, 64, device=dev)
+    wide[:, ::2] = residual
+    got = norm8(block, wide[:, ::2], gate=gate, pre_weight=pre[0], out=wide.view(-1)[:128].view(4, 32))
+    assert torch.equal(got[0], want[0])
+    x, w, ws = rand(5, 4, 32).to(dev), torch.ones(32, 32, dtype=torch.int8, device=dev), rand(6, 32).to(dev)
+    want = int8_linear(x, w, ws)
+    assert torch.equal(int8_linear(x, w, ws, out=x), want)
+    plan = plan_for(dev)
+    one = rand(7, 6 * 8 + plan.capacity * 8).to(dev)
+    x = one[:48].view(6, 8)
+    want = t.sort_tokens(x.clone(), plan)
+    rows = t.sort_tokens(x, plan, out=one[48:].view(-1, 8).zero_())
+    assert torch.equal(rows, want)
