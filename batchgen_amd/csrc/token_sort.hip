@@ -329,8 +329,9 @@ extern "C" int bgmoe_token_unsort_backward(const void* d_out, const void* rows, 
   BGMOE_REQUIRE(num_local_experts >= 1, "token_unsort_backward: no experts");
   if (!d_rows && !d_weights) return BGMOE_OK;
   if (n == 0 && num_rows == 0) return BGMOE_OK;
-  BGMOE_REQUIRE(counts && cu_seqlens && (n == 0 || (d_out && topk_pos)), "token_unsort_backward: null pointer");
-  BGMOE_REQUIRE(n == 0 || !d_weights || rows, "token_unsort_backward: the weights' gradient needs the rows");
+  // rows without elements may have no address; their weights' gradient is 0
+  BGMOE_REQUIRE(counts && cu_seqlens && (n == 0 || ((d_out || h == 0) && topk_pos)), "token_unsort_backward: null pointer");
+  BGMOE_REQUIRE(n == 0 || !d_weights || rows || h == 0, "token_unsort_backward: the weights' gradient needs the rows");
   const int size = dtype == BGMOE_DT_FP32 ? 4 : 2;
   const Rest rest{counts, cu_seqlens, num_local_experts, num_rows, (int64_t)h * size, (uint8_t*)d_rows};
 #define BGMOE_CALL(T) \

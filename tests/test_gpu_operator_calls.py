@@ -285,3 +285,19 @@ def test_outputs_that_may_be_an_operand(dev):
     want = t.sort_tokens(x.clone(), plan)
     rows = t.sort_tokens(x, plan, out=one[48:].view(-1, 8).zero_())
     assert torch.equal(rows, want)
+
+
+# ---- sizes ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n", [0, 1, 6])
+def test_rows_of_width_zero(dev, n):
+    t, plan = sort_api(), plan_for(dev, n=n)
+    x = torch.zeros(n, 0, device=dev, requires_grad=True)
+    w = rand(1, n, 2).to(dev).requires_grad_(True)
+    rows = t.sort_tokens(x, plan)
+    out = t.unsort_tokens(rows, plan, w)
+    assert rows.shape == (plan.capacity, 0) and out.shape == (n, 0)
+    gx, gw = torch.autograd.grad(out.sum(), (x, w))
+    assert gx.shape == (n, 0) and gw.shape == (n, 2) and not bool(gw.any())
+    held = torch.zeros(plan.capacity, 0, device=dev, requires_grad=True)
+    (g,) = torch.autograd.grad(t.unsort_tokens(held, plan, w.detach()).sum(), held)
+    assert g.shape == (plan.capacity, 0)
