@@ -113,13 +113,15 @@ def _sort_backward(ctx, d_rows):
 
 def _unsort_backward(ctx, d_out):
     rows, weights = ctx.saved_tensors
-    plan, d_out = ctx.plan, d_out.contiguous()
-    d_rows = torch.empty_like(rows) if ctx.needs_input_grad[0] else None
-    d_weights = torch.empty_like(weights) if weights is not None and ctx.needs_input_grad[1] else None
-    if d_rows is not None or d_weights is not None:
-        ck.launch(rows.device, lib().bgmoe_token_unsort_backward, ptr(d_out), ptr(rows), ck.dtype_code(rows, "rows"),
-                  ptr(plan.topk_pos), ptr(weights), plan.num_tokens, plan.top_k, rows.size(1), ptr(plan.meta),
-                  ptr(plan.meta) + 4 * plan.num_experts, plan.num_experts, plan.capacity, ptr(d_rows), ptr(d_weights))
+    plan, d_out, h = ctx.plan, d_out.contiguous(), d_out.size(1)
+    d_rows = d_weights = None
+    if ctx.needs_input_grad[0]:
+        d_rows = torch.empty((plan.capacity, h), dtype=d_out.dtype, device=d_out.device)
+    if ctx.needs_input_grad[1]:
+        d_weights = torch.empty((plan.num_tokens, plan.top_k), dtype=torch.float32, device=d_out.device)
+    ck.launch(d_out.device, lib().bgmoe_token_unsort_backward, ptr(d_out), ptr(rows), ck.dtype_code(d_out, "d_out"),
+              ptr(plan.topk_pos), ptr(weights), plan.num_tokens, plan.top_k, h, ptr(plan.meta),
+              ptr(plan.meta) + 4 * plan.num_experts, plan.num_experts, plan.capacity, ptr(d_rows), ptr(d_weights))
     return d_rows, d_weights
 
 
@@ -143,7 +145,8 @@ class _Unsort(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, plan):
         ctx.plan = plan
-        ctx.save_for_backward(rows, weights)
+        # the rows' gradient reads the weights, the weights' gradient the rows
+        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, weights if ctx.needs_input_grad[0] else None)
         return _run_unsort(rows, plan, weights, None)
 
     @staticmethod

@@ -301,3 +301,23 @@ def test_rows_of_width_zero(dev, n):
     held = torch.zeros(plan.capacity, 0, device=dev, requires_grad=True)
     (g,) = torch.autograd.grad(t.unsort_tokens(held, plan, w.detach()).sum(), held)
     assert g.shape == (plan.capacity, 0)
+
+
+# ---- memory held for the backward pass -------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows_need,weights_need", [(True, None), (True, False), (False, True), (True, True)])
+def test_unsort_saves_what_its_gradient_reads(dev, rows_need, weights_need):
+    t, plan = sort_api(), plan_for(dev)
+    rows = rand(1, plan.capacity, 8).to(dev).requires_grad_(rows_need)
+    w = None if weights_need is None else rand(2, 6, 2).to(dev).requires_grad_(weights_need)
+    held = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: held.append(v.shape) or v, lambda v: v):
+        out = t.unsort_tokens(rows, plan, w)
+    assert held == ([rows.shape] if weights_need else []) + ([w.shape] if w is not None and rows_need else [])
+    c = rand(3, 6, 8).to(dev)
+    leaves = [v for v in (rows, w) if v is not None and v.requires_grad]
+    grads = torch.autograd.grad(out, leaves, c)
+    every = [rows.detach().requires_grad_(True), rand(2, 6, 2).to(dev) if w is None else w.detach().clone()]
+    every[1].requires_grad_(True)
+    want = torch.autograd.grad(t.unsort_tokens(every[0], plan, None if w is None else every[1]), every, c, allow_unused=True)
+    for g, v in zip(grads, leaves):
+        assert torch.equal(g, want[0 if v is rows else 1])
