@@ -735,16 +735,25 @@ constexpr int kStreamRows = 32;
 constexpr int kSmallTileRows = 160;
 
 template <bool FUSED, typename TL>
-int run_tiled(const char* what, const Int8Args& a, int groups, hipStream_t st) {
+int64_t tiled_blocks(const Int8Args& a, int groups) {
   // a bound on the m-tiles of groups above the streaming limit, whatever the counts
   const int64_t m_tiles = a.seqlens ? a.m / TL::M + min((int64_t)groups, a.m / (kStreamRows + 1)) : (a.m + TL::M - 1) / TL::M;
   constexpr int kCols = FUSED ? TL::W / 2 : TL::W;
-  const int64_t blocks = (m_tiles * ((a.n + kCols - 1) / kCols) + 7) / 8 * 8;
-  BGMOE_REQUIRE(blocks <= 1 << 22, "%s: m=%lld x n=%d is too large for one launch", what, (long long)a.m, a.n);
+  return (m_tiles * ((a.n + kCols - 1) / kCols) + 7) / 8 * 8;
+}
+constexpr int64_t kMaxBlocks = 1 << 22;
+constexpr int kMaxN = 1 << 22;
+
+template <bool FUSED, typename TL>
+int run_tiled(const char* what, const Int8Args& a, int groups, hipStream_t st) {
+  const int64_t blocks = tiled_blocks<FUSED, TL>(a, groups);
+  BGMOE_REQUIRE(blocks <= kMaxBlocks, "%s: m=%lld x n=%d is too large for one launch", what, (long long)a.m, a.n);
   hipLaunchKernelGGL((int8_tiled_kernel<FUSED, TL>), dim3((unsigned)blocks), dim3(TL::kThreads), TL::kRing, st, a, groups,
                      kStreamRows);
   return bgmoe_check_launch(what);
 }
+
+bool small_tiles(const Int8Args& a, int groups) { return a.m <= (int64_t)kSmallTileRows * groups; }
 
 template <bool FUSED>
 int run_stream(const char* what, const Int8Args& a, int groups, hipStream_t st) {
@@ -762,8 +771,7 @@ int run_grouped(const char* what, const Int8Args& a, int groups, hipStream_t st)
   s.past_cache = (int64_t)groups * a.n * a.k * (FUSED ? 2 : 1) > (256LL << 20);
   const int rc = run_stream<FUSED>(what, s, groups, st);
   if (rc != BGMOE_OK || a.m <= kStreamRows) return rc;
-  return a.m <= (int64_t)kSmallTileRows * groups ? run_tiled<FUSED, Small>(what, a, groups, st)
-                                                 : run_tiled<FUSED, Large>(what, a, groups, st);
+  return small_tiles(a, groups) ? run_tiled<FUSED, Small>(what, a, groups, st) : run_tiled<FUSED, Large>(what, a, groups, st);
 }
 
 template <int RT, int MT>
@@ -818,7 +826,7 @@ int run_dense(const char* what, const Int8Args& a, hipStream_t st) {
 }
 
 int run_gemm(const char* what, const Int8Args& a, int groups, hipStream_t st) {
-  BGMOE_REQUIRE(a.n <= 1 << 22, "%s: n=%d is too wide", what, a.n);
+  BGMOE_REQUIRE(a.n <= kMaxN, "%s: n=%d is too wide", what, a.n);
   BgmoeProf prof(BGMOE_K_INT8_GEMM, st);
   if (a.seqlens == nullptr) return run_dense(what, a, st);
   return a.w1 ? run_grouped<true>(what, a, groups, st) : run_grouped<false>(what, a, groups, st);
@@ -929,6 +937,12 @@ static int grouped(const char* what, Int8Args& a, int groups, int out_dtype, bgm
   BGMOE_REQUIRE(((uintptr_t)a.x | (uintptr_t)a.w0 | (uintptr_t)a.w0_group | (uintptr_t)a.w1 | (uintptr_t)a.w1_group) % 16 == 0,
                 "%s: x, weights and their group strides must be multiples of 16 bytes", what);
   a.ldx = a.k; a.ldo = a.n; a.out_dtype = out_dtype;
+  // before the first of the two launches, so that a refused call has written nothing
+  const bool small = small_tiles(a, groups);
+  const int64_t blocks = a.w1 ? (small ? tiled_blocks<true, Small>(a, groups) : tiled_blocks<true, Large>(a, groups))
+                              : (small ? tiled_blocks<false, Small>(a, groups) : tiled_blocks<false, Large>(a, groups));
+  BGMOE_REQUIRE(a.n <= kMaxN && (a.m <= kStreamRows || blocks <= kMaxBlocks), "%s: m=%lld x n=%d is too large for one launch", what,
+                (long long)a.m, a.n);
   rc = ensure_init();
   if (rc != BGMOE_OK) return rc;
   return run_gemm(what, a, groups, bgmoe_stream(stream));
