@@ -321,3 +321,90 @@ def test_unsort_saves_what_its_gradient_reads(dev, rows_need, weights_need):
     want = torch.autograd.grad(t.unsort_tokens(every[0], plan, None if w is None else every[1]), every, c, allow_unused=True)
     for g, v in zip(grads, leaves):
         assert torch.equal(g, want[0 if v is rows else 1])
+
+
+# ---- many groups, large weight stacks --------------------------------------------------------------------------------
+def int8_operands(dev, rows, e, n, k, seed):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    w = torch.empty(e, n, k, dtype=torch.int8, device=dev)
+    for part in w:                                        # one expert at a time: what randint makes is copied
+        part.copy_(torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8, device=dev))
+    return (torch.randint(-128, 128, (rows, k), generator=g, dtype=torch.int8, device=dev),
+            0.5 + torch.rand(rows, generator=g, device=dev), w, 0.5 + torch.rand(e, n, generator=g, device=dev))
+
+
+def offsets(counts, dev):
+    c = torch.tensor(counts, dtype=torch.int32)
+    cu = torch.zeros(len(counts) + 1, dtype=torch.int32)
+    cu[1:] = c.cumsum(0)
+    return c.to(dev), cu.to(dev), cu.tolist()
+
+
+def check_groups(dev, counts, n, k, seed, groups=None):
+    """Grouped and fused products against the dense product and the fused product of each expert by itself: the same
+    integers, scaled by the same operations."""
+    from batchgen_amd.moe.grouped_int8_moe import int8_fused_s1, int8_grouped_gemm
+    from batchgen_amd.quantization.int8 import int8_linear
+    c, cu, at = offsets(counts, dev)
+    x, xs, w, ws = int8_operands(dev, at[-1], len(counts), n, k, seed)
+    got = int8_grouped_gemm(x, xs, w, ws, c, cu, out_dtype=torch.float32)
+    half = n // 2
+    fused = int8_fused_s1(x, xs, w[:, :half], ws[:, :half], w[:, half:2 * half], ws[:, half:2 * half], c, cu, out_dtype=torch.float32)
+    for g in range(len(counts)) if groups is None else groups:
+        sl = slice(at[g], at[g + 1])
+        if not counts[g]:
+            continue
+        assert torch.equal(got[sl], int8_linear(x[sl], w[g], ws[g], x_scale=xs[sl], out_dtype=torch.float32)), (g, counts[g])
+        one, zero = offsets([counts[g]], dev)[:2]
+        alone = int8_fused_s1(x[sl], xs[sl], w[g:g + 1, :half], ws[g:g + 1, :half], w[g:g + 1, half:2 * half],
+                              ws[g:g + 1, half:2 * half], one, zero, out_dtype=torch.float32)
+        assert torch.equal(fused[sl], alone), (g, counts[g])
+
+
+def test_against_the_definition_once(dev):
+    """What the comparisons of this section rest on: the dense product and one group's fused product against 64 bits."""
+    from batchgen_amd.moe.grouped_int8_moe import int8_fused_s1
+    from batchgen_amd.quantization.int8 import int8_linear
+    from tests import operator_ref as ref
+    x, xs, w, ws = int8_operands(dev, 40, 1, 66, 80, 1)
+    one, cu, _ = offsets([40], dev)
+    x64, w64 = x.cpu().double() * xs.cpu().double()[:, None], w[0].cpu().double() * ws[0].cpu().double()[:, None]
+    want = x64 @ w64.t()
+    got = int8_linear(x, w[0], ws[0], x_scale=xs, out_dtype=torch.float32)
+    # sum to fp32 and two scalings: three half steps (fp64's own error is 2^-29 of one)
+    ref.assert_within(got, want, 4 * ref.U32 * want.abs() + 1e-6 * ref.U32, "dense")
+    fused = int8_fused_s1(x, xs, w[:, :33], ws[:, :33], w[:, 33:], ws[:, 33:], one, cu, out_dtype=torch.float32)
+    g64, u64 = want[:, :33], want[:, 33:]
+    h64 = g64 * torch.sigmoid(g64) * u64
+    tol = (4 * g64.abs() + 16) * ref.U32 * h64.abs() + torch.finfo(torch.float32).smallest_normal
+    ref.assert_within(fused, h64, tol + ref.half_step(torch.float32, h64.abs() + tol), "fused")
+
+
+@pytest.mark.parametrize("groups", [64, 65, 200, 1024])
+def test_many_groups(dev, groups):
+    """More groups than the lanes that scan their tile counts: the last of each 64 and the first of the next hold rows."""
+    counts = [0] * groups
+    for i, v in ((0, 33), (1, 1), (63, 130), (64, 40), (65, 17), (127, 35), (128, 70), (199, 34), (511, 3), (960, 36), (1023, 129)):
+        if i < groups:
+            counts[i] = v
+    counts[-1] = max(counts[-1], 34)
+    check_groups(dev, counts, 34, 48, 7)
+
+
+def test_many_groups_in_the_large_tiles_beyond_the_emulator(dev):
+    g = torch.Generator().manual_seed(8)
+    counts = (torch.randint(0, 420, (130,), generator=g) * (torch.rand(130, generator=g) < 0.9)).tolist()
+    assert sum(counts) > 160 * len(counts)
+    check_groups(dev, counts, 260, 272, 9)
+
+
+def test_weight_stacks_beyond_the_last_level_cache(dev):
+    """More than 256 MB of weights are streamed past the cache: whole stages and a K tail, one and two token tiles."""
+    check_groups(dev, [0, 1, 16, 17, 32], 4001, 16016, 10)
+    check_groups(dev, [40, 1, 0, 65, 32], 4001, 16016, 11)
+
+
+def test_weight_stacks_beyond_32_bits(dev):
+    for counts in ([0, 2, 0, 20], [1, 0, 0, 70]):         # the last expert's weights start at 4.9e9 bytes
+        check_groups(dev, counts, 100000, 16384, 12)
+        torch.cuda.empty_cache()
