@@ -89,6 +89,8 @@ RESOURCE_GATES = {
     "gemm_fp8_skinny.hip": dict(kernel="fp8_skinny_kernel", min_occupancy=2),
     "gemm_mxfp4_skinny.hip": dict(kernel="mxfp4_skinny_kernel", min_occupancy=2),
     "gemm_fp8_streamk.hip": dict(kernel="fp8_streamk_kernel"),
+    # the int8 products: their rings' waits count loads alone, and the 256-row tile uses every register it may have
+    "gemm_int8.hip": dict(kernel="int8_", min_occupancy=2),
     "gemm_fp8_tiled_k64.hip": dict(kernel="fp8_tiled_k64_kernel", max_vgprs=256, max_agprs=0,
                                    max_static_lds=163840 - 4 * (32768 + 1024), min_occupancy=2),
 }
