@@ -44,7 +44,7 @@ void emu_install_handlers();
 namespace emu {
 namespace {
 
-enum Op { OP_NONE = 0, OP_SYNC, OP_SHFL, OP_BALLOT, OP_RFL, OP_RLANE, OP_MFMA16_F8, OP_MFMA32_F8, OP_MFMA16_BF16, OP_MFMA16_I8, OP_MFMA32_I8, OP_DPP, OP_BARRIER };
+enum Op { OP_NONE = 0, OP_SYNC, OP_SHFL, OP_BALLOT, OP_RFL, OP_RLANE, OP_MFMA16_F8, OP_MFMA32_F8, OP_MFMA16_BF16, OP_MFMA16_I8, OP_DPP, OP_BARRIER };
 
 struct Pending { const uint8_t* src; uint8_t* dst; unsigned bytes; };
 
@@ -237,23 +237,19 @@ void perform(Fiber* wave, const std::vector<int>& who) {
         }
       break;
     }
-    case OP_MFMA16_I8:
-    case OP_MFMA32_I8: {
-      // R = 16 or 32 rows: lane l = row l % R, K bytes 16 (l / R) .. + 15 of both operands; 32-bit sums that wrap;
-      // D as the f8 forms of the same size
+    case OP_MFMA16_I8: {
+      // lane l = row l % 16, K bytes 16 (l / 16) .. + 15 of both operands; 32-bit sums that wrap; D as the f8 form
       if (who.size() != 64) die("matrix instruction with %zu of 64 lanes", who.size());
-      const int R = op == OP_MFMA16_I8 ? 16 : 32, K = 1024 / R;
-      static int8_t A[32][64], B[32][64];
+      static int8_t A[16][64], B[16][64];
       for (int l = 0; l < 64; ++l)
         for (int k = 0; k < 16; ++k) {
-          A[l % R][16 * (l / R) + k] = reinterpret_cast<const int8_t*>(wave[l].in)[k];
-          B[l % R][16 * (l / R) + k] = reinterpret_cast<const int8_t*>(wave[l].in + 4)[k];
+          A[l % 16][16 * (l / 16) + k] = reinterpret_cast<const int8_t*>(wave[l].in)[k];
+          B[l % 16][16 * (l / 16) + k] = reinterpret_cast<const int8_t*>(wave[l].in + 4)[k];
         }
       for (int l = 0; l < 64; ++l)
-        for (int v = 0; v < (R == 16 ? 4 : 16); ++v) {
-          const int i = R == 16 ? 4 * (l >> 4) + v : 8 * (v >> 2) + 4 * (l >> 5) + (v & 3), j = l % R;
+        for (int v = 0; v < 4; ++v) {
           uint32_t s = wave[l].in[8 + v];
-          for (int k = 0; k < K; ++k) s += (uint32_t)((int)A[i][k] * (int)B[j][k]);
+          for (int k = 0; k < 64; ++k) s += (uint32_t)((int)A[4 * (l >> 4) + v][k] * (int)B[l % 16][k]);
           wave[l].out[v] = s;
         }
       break;
@@ -482,13 +478,6 @@ __attribute__((noinline)) void mfma_16x16x64_i8(const int32_t* a4, const int32_t
   memcpy(g_cur->in + 8, c4, 16);
   rendezvous(OP_MFMA16_I8, __builtin_return_address(0));
   memcpy(d4, g_cur->out, 16);
-}
-__attribute__((noinline)) void mfma_32x32x32_i8(const int32_t* a4, const int32_t* b4, const int32_t* c16, int32_t* d16) {
-  memcpy(g_cur->in, a4, 16);
-  memcpy(g_cur->in + 4, b4, 16);
-  memcpy(g_cur->in + 8, c16, 64);
-  rendezvous(OP_MFMA32_I8, __builtin_return_address(0));
-  memcpy(d16, g_cur->out, 64);
 }
 
 void async_load(const void* base, uint32_t lane_off, uint32_t lds_base, unsigned bytes, bool uniform_base) {

@@ -73,7 +73,6 @@ void mfma_16x16x128_f8(const int32_t* a8, const int32_t* b8, const float* c4, fl
 void mfma_32x32x64_f8(const int32_t* a8, const int32_t* b8, const float* c16, float* d16);
 void mfma_16x16x32_bf16(const uint16_t* a8, const uint16_t* b8, const float* c4, float* d4);
 void mfma_16x16x64_i8(const int32_t* a4, const int32_t* b4, const int32_t* c4, int32_t* d4);
-void mfma_32x32x32_i8(const int32_t* a4, const int32_t* b4, const int32_t* c16, int32_t* d16);
 // asynchronous global -> LDS loads (see bgmoe_async.h of this directory)
 void async_load(const void* base, uint32_t lane_off, uint32_t lds_base, unsigned bytes, bool uniform_base = true);
 void wait_vm(int n);
@@ -239,7 +238,6 @@ static inline emu_floatx4 emu_mfma_bf16(emu_bf16x8 a, emu_bf16x8 b, emu_floatx4 
   return d;
 }
 typedef int emu_intx4 __attribute__((ext_vector_type(4)));
-typedef int emu_intx16 __attribute__((ext_vector_type(16)));
 static inline emu_intx4 emu_mfma_i8_16(emu_intx4 a, emu_intx4 b, emu_intx4 c, int = 0, int = 0, int = 0) {
   int32_t av[4], bv[4], cv[4], dv[4];
   memcpy(av, &a, 16); memcpy(bv, &b, 16); memcpy(cv, &c, 16);
@@ -248,16 +246,7 @@ static inline emu_intx4 emu_mfma_i8_16(emu_intx4 a, emu_intx4 b, emu_intx4 c, in
   memcpy(&d, dv, 16);
   return d;
 }
-static inline emu_intx16 emu_mfma_i8_32(emu_intx4 a, emu_intx4 b, emu_intx16 c, int = 0, int = 0, int = 0) {
-  int32_t av[4], bv[4], cv[16], dv[16];
-  memcpy(av, &a, 16); memcpy(bv, &b, 16); memcpy(cv, &c, 64);
-  emu::mfma_32x32x32_i8(av, bv, cv, dv);
-  emu_intx16 d;
-  memcpy(&d, dv, 64);
-  return d;
-}
 #define __builtin_amdgcn_mfma_i32_16x16x64_i8(...) emu_mfma_i8_16(__VA_ARGS__)
-#define __builtin_amdgcn_mfma_i32_32x32x32_i8(...) emu_mfma_i8_32(__VA_ARGS__)
 // (the format and scale arguments of the f8f6f4 forms are 0 everywhere in this library: e4m3 x e4m3, unit scales)
 // (variadic: an operand written as a braced vector literal holds commas)
 #define __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(...) emu_mfma_16x16x128(__VA_ARGS__)
