@@ -72,8 +72,8 @@ def _forward(c, block, residual, post, gate, pre, y, normed, q, q_scale, inv_pos
                   ptr(q_scale), inv_post, inv_pre)
 
 
-def _backward(ctx, d_y, d_normed):
-    block, residual, post, gate, pre, inv = ctx.saved_tensors
+def _backward(ctx, saved, d_y, d_normed):
+    block, residual, post, gate, pre, inv = saved
     c, need = ctx.call, ctx.needs_input_grad
     if d_y is None and d_normed is None:
         return None, None, None, None, None, None
@@ -98,9 +98,9 @@ def _backward(ctx, d_y, d_normed):
     return (*grads, None)
 
 
-def _tied_to_sources(ctx, d_y, d_normed, grads):
+def _tied_to_sources(saved, d_y, d_normed, grads):
     """The gradients of (block, residual, post, gate, pre) with what each of them depends on."""
-    block, residual, post, gate, pre, _ = ctx.saved_tensors
+    block, residual, post, gate, pre, _ = saved
     if d_normed is not None:                              # through the second norm: on everything, but linearly on pre
         every = (block, residual, post, gate, d_y, d_normed)
         sources = ((*every, pre),) * 4 + (every,)
@@ -124,11 +124,12 @@ class _GatedNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_y, d_normed):
+        saved = ctx.saved_tensors                         # once: checkpointing recomputes them at the first access
         if not torch.is_grad_enabled():
-            return _backward(ctx, d_y, d_normed)
+            return _backward(ctx, saved, d_y, d_normed)
         with torch.no_grad():                             # a graph of the backward pass is being recorded
-            grads = _backward(ctx, d_y, d_normed)
-        return (*_tied_to_sources(ctx, d_y, d_normed, grads[:5]), None)
+            grads = _backward(ctx, saved, d_y, d_normed)
+        return (*_tied_to_sources(saved, d_y, d_normed, grads[:5]), None)
 
 
 def _contiguous(*tensors):

@@ -111,8 +111,7 @@ def _sort_backward(ctx, d_rows):
     return _run_unsort(d_rows.contiguous(), ctx.plan, None, None)
 
 
-def _unsort_backward(ctx, d_out):
-    rows, weights = ctx.saved_tensors
+def _unsort_backward(ctx, d_out, rows, weights):
     plan, d_out, h = ctx.plan, d_out.contiguous(), d_out.size(1)
     d_rows = d_weights = None
     if ctx.needs_input_grad[0]:
@@ -151,11 +150,11 @@ class _Unsort(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_out):
+        rows, weights = ctx.saved_tensors                 # once: checkpointing recomputes them at the first access
         if not torch.is_grad_enabled():
-            return (*_unsort_backward(ctx, d_out), None)
+            return (*_unsort_backward(ctx, d_out, rows, weights), None)
         with torch.no_grad():
-            d_rows, d_weights = _unsort_backward(ctx, d_out)
-        rows, weights = ctx.saved_tensors
+            d_rows, d_weights = _unsort_backward(ctx, d_out, rows, weights)
         return (no_second_gradient("unsort_tokens", d_rows, d_out, weights),
                 no_second_gradient("unsort_tokens", d_weights, d_out, rows), None)
 

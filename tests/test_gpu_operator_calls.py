@@ -408,3 +408,20 @@ def test_weight_stacks_beyond_32_bits(dev):
     for counts in ([0, 2, 0, 20], [1, 0, 0, 70]):         # the last expert's weights start at 4.9e9 bytes
         check_groups(dev, counts, 100000, 16384, 12)
         torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_checkpointed_block(dev, create_graph):
+    """Under torch's checkpointing a backward pass may read what was saved only once."""
+    from torch.utils.checkpoint import checkpoint
+    t, plan = sort_api(), plan_for(dev)
+    v = norm_leaves(dev, h=8)
+    x, w = rand(1, 6, 8).to(dev).requires_grad_(True), rand(2, 6, 2).to(dev).requires_grad_(True)
+
+    def block(x_, w_):
+        out = t.unsort_tokens(t.sort_tokens(x_, plan), plan, w_)
+        return norm_of(dict(v, block=out[:4]))[1]
+    leaves = (x, w, v["post"], v["gate"])
+    want = torch.autograd.grad(block(x, w).sum(), leaves)
+    got = torch.autograd.grad(checkpoint(block, x, w, use_reentrant=False).sum(), leaves, create_graph=create_graph)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
