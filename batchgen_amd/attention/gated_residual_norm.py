@@ -23,6 +23,14 @@ MAX_HIDDEN = 16384
 _NONE, _CHANNEL, _TOKEN, _FULL = range(4)
 
 
+def _constant(value, name):
+    """residual_scale and eps are numbers: a tensor's derivative would be lost."""
+    if isinstance(value, torch.Tensor):
+        ck.no_tangent(f"gated_residual_rmsnorm({name}=)", value)
+        if value.requires_grad and torch.is_grad_enabled():
+            ck.fail(f"{name} has no gradient: pass a number (a learned scale can be the gate)")
+
+
 class _Call:
     """The checked operands of one call: 2-D views, codes and flags of the C ABI."""
     __slots__ = ("code", "rows", "h", "gate_mode", "param_fp32", "scale", "eps", "device")
@@ -40,6 +48,9 @@ class _Call:
         h = self.h = block.size(-1)
         self.rows = block.numel() // h
         self.device = block.device
+        if type(scale) is not float or type(eps) is not float:
+            _constant(scale, "residual_scale")
+            _constant(eps, "eps")
         self.scale, self.eps = float(scale), float(eps)
         self.param_fp32 = 0
         for bit, p, name in ((1, post, "post_weight"), (2, gate, "gate"), (4, pre, "pre_weight")):

@@ -425,3 +425,21 @@ def test_checkpointed_block(dev, create_graph):
     want = torch.autograd.grad(block(x, w).sum(), leaves)
     got = torch.autograd.grad(checkpoint(block, x, w, use_reentrant=False).sum(), leaves, create_graph=create_graph)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("name", ["residual_scale", "eps"])
+def test_numbers_that_require_a_gradient_are_refused(dev, name):
+    from torch.autograd import forward_ad
+    block, residual, pre = rand(1, 4, 8).to(dev), rand(2, 4, 8).to(dev), rand(3, 8).to(dev)
+    value = torch.tensor(0.5, device=dev)
+    for f in (norm_api().gated_residual_rmsnorm, norm_api().gated_residual_rmsnorm_int8_quant):
+        want = f(block, residual, pre_weight=pre, **{name: 0.5})
+        for plain in (value, value.cpu(), 0.5):           # a constant is a number
+            assert all(torch.equal(a, b) for a, b in zip(f(block, residual, pre_weight=pre, **{name: plain}), want))
+        assert f(block, residual, pre_weight=pre, **{name: 1})[0].shape == block.shape
+        with pytest.raises(RuntimeError, match="has no gradient"):
+            f(block, residual, pre_weight=pre, **{name: value.clone().requires_grad_(True)})
+        with pytest.raises(RuntimeError, match="forward-mode"), forward_ad.dual_level():
+            f(block, residual, pre_weight=pre, **{name: forward_ad.make_dual(value, value)})
+        with torch.no_grad():
+            assert torch.equal(f(block, residual, pre_weight=pre, **{name: value.clone().requires_grad_(True)})[0], want[0])
