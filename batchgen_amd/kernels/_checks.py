@@ -90,11 +90,13 @@ def writable(name: str, *outs):
                 fail(f"{name} writes its output without a gradient: the tensor it writes must not require one in grad mode")
 
 
-def _end(t: torch.Tensor, start: int) -> int:
-    """The address behind the last element of ``t``."""
+def _reaches(t: torch.Tensor, address: int) -> bool:
+    """Whether the memory of ``t``, to the end of its last element, reaches beyond ``address``."""
     if t.is_contiguous():
-        return start + t.nbytes
-    return start + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else start
+        size = t.nbytes
+    else:                                               # (not empty: an empty tensor is contiguous)
+        size = (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    return t.data_ptr() + size > address
 
 
 def apart(name: str, out: torch.Tensor, *operands, same_ok=()):
@@ -103,15 +105,12 @@ def apart(name: str, out: torch.Tensor, *operands, same_ok=()):
     start = out.data_ptr()
     end = start + out.nbytes                            # (outputs are contiguous)
     for t in operands:
-        if t is not None:
-            p = t.data_ptr()
-            if p < end and _end(t, p) > start and p != 0:
-                fail(f"{name}: the output must not share memory with an operand")
+        if t is not None and t.data_ptr() < end and _reaches(t, start):
+            fail(f"{name}: the output must not share memory with an operand")
     for t in same_ok:
-        if t is not None:
-            p = t.data_ptr()
-            if p < end and _end(t, p) > start and p != 0 and not (p == start and t.is_contiguous() and t.nbytes == out.nbytes):
-                fail(f"{name}: the output must be an operand's whole memory or none of it")
+        if t is not None and t.data_ptr() < end and _reaches(t, start) and \
+                not (t.data_ptr() == start and t.is_contiguous() and t.nbytes == out.nbytes):
+            fail(f"{name}: the output must be an operand's whole memory or none of it")
 
 
 def written(*outs):

@@ -76,7 +76,8 @@ def int8_grouped_gemm(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tens
     or ``out`` says otherwise; rows of no expert keep what ``out`` held, which shares no memory with the operands)."""
     no_grad_needed("int8_grouped_gemm", x_scale, weight_scale)
     held = out
-    ck.writable("int8_grouped_gemm", held)
+    if held is not None:
+        ck.writable("int8_grouped_gemm", held)
     e = weight.size(0) if isinstance(weight, torch.Tensor) and weight.dim() == 3 else 0
     m, k = _rows(x, x_scale, seqlens, cu_seqlens, e)
     _weight(x, weight, weight_scale, k, "weight")
@@ -88,7 +89,8 @@ def int8_grouped_gemm(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tens
         ck.launch(x.device, lib().bgmoe_int8_grouped_gemm, ptr(x), ptr(x_scale), ptr(weight), weight.stride(0),
                   ptr(weight_scale), weight_scale.stride(0), ptr(seqlens), ptr(cu_seqlens), e, m, n, k, ptr(out),
                   code)
-        ck.written(held)
+        if held is not None:
+            ck.written(held)
     return out
 
 
@@ -99,7 +101,8 @@ def int8_fused_s1(x: torch.Tensor, x_scale: torch.Tensor, gate_weight: torch.Ten
     ``up_weight`` int8 ``[E, N, K]``."""
     no_grad_needed("int8_fused_s1", x_scale, gate_scale, up_scale)
     held = out
-    ck.writable("int8_fused_s1", held)
+    if held is not None:
+        ck.writable("int8_fused_s1", held)
     e = gate_weight.size(0) if isinstance(gate_weight, torch.Tensor) and gate_weight.dim() == 3 else 0
     m, k = _rows(x, x_scale, seqlens, cu_seqlens, e)
     _weight(x, gate_weight, gate_scale, k, "gate_weight")
@@ -114,5 +117,6 @@ def int8_fused_s1(x: torch.Tensor, x_scale: torch.Tensor, gate_weight: torch.Ten
         ck.launch(x.device, lib().bgmoe_int8_fused_s1, ptr(x), ptr(x_scale), ptr(gate_weight), gate_weight.stride(0),
                   ptr(gate_scale), gate_scale.stride(0), ptr(up_weight), up_weight.stride(0), ptr(up_scale),
                   up_scale.stride(0), ptr(seqlens), ptr(cu_seqlens), e, m, n, k, ptr(out), code)
-        ck.written(held)
+        if held is not None:
+            ck.written(held)
     return out

@@ -182,7 +182,8 @@ def sort_tokens(x: torch.Tensor, plan: TokenSortPlan, out: Optional[torch.Tensor
         ck.writable("sort_tokens", out)
         ck.apart("sort_tokens", out, x, plan.topk_pos, plan.meta)
     rows = _run_sort(x, plan, out)
-    ck.written(out)
+    if out is not None:
+        ck.written(out)
     return rows
 
 
@@ -216,5 +217,6 @@ def unsort_tokens(rows: torch.Tensor, plan: TokenSortPlan, weights: Optional[tor
         ck.writable("unsort_tokens", out)
         ck.apart("unsort_tokens", out, rows, weights, plan.topk_pos, plan.meta)
     tokens = _run_unsort(rows, plan, weights, out)
-    ck.written(out)
+    if out is not None:
+        ck.written(out)
     return tokens

@@ -76,7 +76,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     ck.gpu(x, "x")
     no_grad_needed("int8_linear", x, x_scale, weight_scale, bias)
     held = out
-    ck.writable("int8_linear", held)
+    if held is not None:
+        ck.writable("int8_linear", held)
     ck.cuda_tensor(x, weight, torch.int8, "weight")
     if weight.dim() != 2 or x.dim() < 1 or x.size(-1) != weight.size(1):
         ck.fail(f"int8_linear: x [..., K] and weight [N, K] do not fit: {tuple(x.shape)}, {tuple(weight.shape)}")
@@ -129,5 +130,6 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         ws = torch.empty(lib().bgmoe_int8_linear_workspace_bytes(m, n, k), dtype=torch.uint8, device=x.device)
         ck.launch(x.device, lib().bgmoe_int8_linear, ptr(x2), x_code, x2.stride(0), ptr(weight), ptr(weight_scale),
                   ptr(bias), m, n, k, ptr(out), code, n, ptr(ws), ws.numel())
-    ck.written(held)
+    if held is not None:
+        ck.written(held)
     return out
