@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version as _increment_version
 
 from .._lib import check
 
@@ -90,13 +91,9 @@ def writable(name: str, *outs):
                 fail(f"{name} writes its output without a gradient: the tensor it writes must not require one in grad mode")
 
 
-def _reaches(t: torch.Tensor, address: int) -> bool:
-    """Whether the memory of ``t``, to the end of its last element, reaches beyond ``address``."""
-    if t.is_contiguous():
-        size = t.nbytes
-    else:                                               # (not empty: an empty tensor is contiguous)
-        size = (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-    return t.data_ptr() + size > address
+def _span(t: torch.Tensor) -> int:
+    """Bytes from the first to the last element of a tensor that is not contiguous (and so not empty)."""
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
 def apart(name: str, out: torch.Tensor, *operands, same_ok=()):
@@ -105,12 +102,16 @@ def apart(name: str, out: torch.Tensor, *operands, same_ok=()):
     start = out.data_ptr()
     end = start + out.nbytes                            # (outputs are contiguous)
     for t in operands:
-        if t is not None and t.data_ptr() < end and _reaches(t, start):
-            fail(f"{name}: the output must not share memory with an operand")
+        if t is not None:
+            p = t.data_ptr()
+            if p < end and p + (t.nbytes if t.is_contiguous() else _span(t)) > start:
+                fail(f"{name}: the output must not share memory with an operand")
     for t in same_ok:
-        if t is not None and t.data_ptr() < end and _reaches(t, start) and \
-                not (t.data_ptr() == start and t.is_contiguous() and t.nbytes == out.nbytes):
-            fail(f"{name}: the output must be an operand's whole memory or none of it")
+        if t is not None:
+            p = t.data_ptr()
+            if p < end and p + (t.nbytes if t.is_contiguous() else _span(t)) > start and \
+                    not (p == start and t.is_contiguous() and t.nbytes == out.nbytes):
+                fail(f"{name}: the output must be an operand's whole memory or none of it")
 
 
 def written(*outs):
@@ -119,7 +120,7 @@ def written(*outs):
     version and cannot be saved.)"""
     for t in outs:
         if t is not None and not t.is_inference():
-            torch.autograd.graph.increment_version(t)
+            _increment_version(t)
 
 
 def launch(device: torch.device, fn, *args):
