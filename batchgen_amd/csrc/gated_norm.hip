@@ -16,8 +16,8 @@
 // Both passes are bound by HBM: a row is held in registers between its sums and its outputs, eight elements per thread
 // and vector, and every operand is read once.  The gradient recomputes y in fp32 from block and residual (the same
 // bytes as reading the stored y, without its rounding).  The sums over rows (w1, w2, a channel gate) are accumulated
-// in registers by blocks that walk many rows, written as one fp32 plane per block and added in block order by a second
-// launch: the same bits every time, no atomics.
+// in LDS (rows wider than 8192: in registers) by blocks that walk many rows, written as one fp32 plane per block and
+// added in block order by a second launch: the same bits every time, no atomics.
 #include "bgmoe_elem.h"
 
 namespace {
@@ -187,7 +187,10 @@ __global__ __launch_bounds__(1024) void gated_norm_kernel(NormArgs a) {
 // sums, so that a CU always has a row (57 KB at h = 7168) on its way while its VALU (about 40 operations per element)
 // works on another.  What the blocks sum over their rows lives in LDS, eight floats per thread and kind (in registers it
 // takes the place of that next row, or of a second block per CU).  Order of the planes: post, pre, gate.
-// ACC_LDS = false (rows wider than LDS holds, h > 8192): accumulators in registers.
+// The two-byte types spill four of the 128 registers that a block of 1024 threads leaves (20 bytes of scratch per lane).
+// ACC_LDS = false (rows wider than LDS holds, h > 8192): accumulators in registers, which do not fit: 350 to 390 bytes of
+// scratch per lane are written and read for every row and bound that form.  4096 x 16384 bf16 667 us (1.2 TB/s), fp32 761
+// (2.1), where 4096 x 8192 takes 103 us (3.9 TB/s) and 201 (4.0).
 template <typename T, int V, bool ACC_LDS, bool NT>
 __global__ __launch_bounds__(1024) void gated_norm_backward_kernel(NormArgs a) {
   extern __shared__ __align__(16) float s_acc[];         // [kind][thread * 8 + i]

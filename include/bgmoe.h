@@ -865,7 +865,7 @@ int bgmoe_token_unsort(const void* rows, int dtype, const int32_t* topk_pos, con
 
 /* Gradients of bgmoe_token_unsort: d_rows[topk_pos[t*k+j]] = weights[t*k+j] * d_out[t] (rows without a pair: 0),
  * d_weights[t*k+j] = <d_out[t], rows[topk_pos[t*k+j]]> in fp32 (0 where the pair has no row).  Either output may be
- * NULL.  No atomics: the same bits every time. */
+ * NULL, and then what only it needs (rows for d_weights, weights for d_rows).  No atomics: the same bits every time. */
 int bgmoe_token_unsort_backward(const void* d_out, const void* rows, int dtype, const int32_t* topk_pos,
                                 const float* weights, int n, int k, int h, const int32_t* counts,
                                 const int32_t* cu_seqlens, int num_local_experts, int64_t num_rows, void* d_rows,
