@@ -98,7 +98,7 @@ def _span(t: torch.Tensor) -> int:
 
 def apart(name: str, out: torch.Tensor, *operands, same_ok=()):
     """Refuses an output whose memory (first to last element) reaches into an operand's: blocks of one launch write the
-    one while others still read the other.  An operand of ``same_ok`` may be the output's memory as a whole."""
+    one while others still read the other.  An operand of ``same_ok`` may be the output's memory, element by element."""
     start = out.data_ptr()
     end = start + out.nbytes                            # (outputs are contiguous)
     for t in operands:
@@ -110,7 +110,7 @@ def apart(name: str, out: torch.Tensor, *operands, same_ok=()):
         if t is not None:
             p = t.data_ptr()
             if p < end and p + (t.nbytes if t.is_contiguous() else _span(t)) > start and \
-                    not (p == start and t.is_contiguous() and t.nbytes == out.nbytes):
+                    not (p == start and t.is_contiguous() and t.nbytes == out.nbytes and t.dtype == out.dtype):
                 fail(f"{name}: the output must be an operand's whole memory or none of it")
 
 

@@ -54,7 +54,7 @@ def _weight(x, w, s, k, name):
         ck.fail(f"{name}_scale must be fp32 {tuple(w.shape[:2])} with contiguous rows, got {tuple(s.shape)}")
 
 
-def _out(x, out, out_dtype, m, n):
+def _out(name, x, out, out_dtype, m, n):
     ck.int32(n, "N")
     dt = out.dtype if out is not None else (out_dtype or torch.bfloat16)
     code = ck.DTYPE_CODE.get(dt)
@@ -65,6 +65,7 @@ def _out(x, out, out_dtype, m, n):
     ck.cuda_tensor(x, out, dt, "out")
     if tuple(out.shape) != (m, n):
         ck.fail(f"out must have the shape {(m, n)}, got {tuple(out.shape)}")
+    ck.writable(name, out)
     return out, code
 
 
@@ -76,13 +77,11 @@ def int8_grouped_gemm(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tens
     or ``out`` says otherwise; rows of no expert keep what ``out`` held, which shares no memory with the operands)."""
     no_grad_needed("int8_grouped_gemm", x_scale, weight_scale)
     held = out
-    if held is not None:
-        ck.writable("int8_grouped_gemm", held)
     e = weight.size(0) if isinstance(weight, torch.Tensor) and weight.dim() == 3 else 0
     m, k = _rows(x, x_scale, seqlens, cu_seqlens, e)
     _weight(x, weight, weight_scale, k, "weight")
     n = weight.size(1)
-    out, code = _out(x, out, out_dtype, m, n)
+    out, code = _out("int8_grouped_gemm", x, out, out_dtype, m, n)
     if m and n:
         if held is not None:
             ck.apart("int8_grouped_gemm", out, x, x_scale, weight, weight_scale, seqlens, cu_seqlens)
@@ -101,8 +100,6 @@ def int8_fused_s1(x: torch.Tensor, x_scale: torch.Tensor, gate_weight: torch.Ten
     ``up_weight`` int8 ``[E, N, K]``."""
     no_grad_needed("int8_fused_s1", x_scale, gate_scale, up_scale)
     held = out
-    if held is not None:
-        ck.writable("int8_fused_s1", held)
     e = gate_weight.size(0) if isinstance(gate_weight, torch.Tensor) and gate_weight.dim() == 3 else 0
     m, k = _rows(x, x_scale, seqlens, cu_seqlens, e)
     _weight(x, gate_weight, gate_scale, k, "gate_weight")
@@ -110,7 +107,7 @@ def int8_fused_s1(x: torch.Tensor, x_scale: torch.Tensor, gate_weight: torch.Ten
     if up_weight.shape != gate_weight.shape:
         ck.fail(f"gate_weight {tuple(gate_weight.shape)} and up_weight {tuple(up_weight.shape)} must have one shape")
     n = gate_weight.size(1)
-    out, code = _out(x, out, out_dtype, m, n)
+    out, code = _out("int8_fused_s1", x, out, out_dtype, m, n)
     if m and n:
         if held is not None:
             ck.apart("int8_fused_s1", out, x, x_scale, gate_weight, gate_scale, up_weight, up_scale, seqlens, cu_seqlens)

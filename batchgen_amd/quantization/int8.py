@@ -33,7 +33,6 @@ def int8_quant_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
     ck.gpu(x, "x")
     no_grad_needed("int8_quant_rows", x)
     held = (out, scale)                                   # the caller's tensors
-    ck.writable("int8_quant_rows", *held)
     code = ck.dtype_code(x, "x")
     if x.dim():
         ck.int32(x.size(-1), "K")
@@ -51,6 +50,7 @@ def int8_quant_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
         ck.cuda_tensor(x, scale, torch.float32, "scale")
         if scale.shape != x.shape[:-1]:
             ck.fail(f"scale must have the shape {tuple(x.shape[:-1])}, got {tuple(scale.shape)}")
+    ck.writable("int8_quant_rows", *held)
     if rows and k == 0:
         ck.fail("int8_quant_rows: rows without elements have no scale")
     if rows:
@@ -76,8 +76,6 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     ck.gpu(x, "x")
     no_grad_needed("int8_linear", x, x_scale, weight_scale, bias)
     held = out
-    if held is not None:
-        ck.writable("int8_linear", held)
     ck.cuda_tensor(x, weight, torch.int8, "weight")
     if weight.dim() != 2 or x.dim() < 1 or x.size(-1) != weight.size(1):
         ck.fail(f"int8_linear: x [..., K] and weight [N, K] do not fit: {tuple(x.shape)}, {tuple(weight.shape)}")
@@ -111,6 +109,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         ck.cuda_tensor(x, out, dt, "out")
         if out.shape != shape:
             ck.fail(f"out must have the shape {tuple(shape)}, got {tuple(out.shape)}")
+        ck.writable("int8_linear", out)
     if m == 0 or n == 0:
         return out
     if quantised:

@@ -246,6 +246,7 @@ def test_outputs_that_share_memory_with_an_operand(dev):
                 lambda: norm8(seam[:4], seam[:4].clone(), pre_weight=pre, out=seam[1:]),
                 lambda: norm8(seam[:4].clone(), seam[1:], pre_weight=pre, out=seam[:4]),
                 lambda: norm8(seam[:1], seam[1:2], pre_weight=pre, out=pre.view(1, 32)),
+                lambda: norm8(seam[:2].half(), seam[1:3].half(), gate=pre, pre_weight=seam[4], out=pre.view(torch.float16).view(2, 32)),
                 lambda: int8_quant_rows(x, out=x.view(torch.int8)[:16].view(64, 16)),
                 lambda: int8_quant_rows(x, scale=x[:4].view(64)),
                 lambda: int8_quant_rows(x[:1, :4], out=ones[:1].view(torch.int8).view(1, 4), scale=ones[:1]),
@@ -443,3 +444,11 @@ def test_numbers_that_require_a_gradient_are_refused(dev, name):
             f(block, residual, pre_weight=pre, **{name: forward_ad.make_dual(value, value)})
         with torch.no_grad():
             assert torch.equal(f(block, residual, pre_weight=pre, **{name: value.clone().requires_grad_(True)})[0], want[0])
+
+
+def test_outputs_that_are_no_tensor_are_refused(dev):
+    for name, outs, call in calls_with_out(dev):
+        for i in range(len(outs)):
+            with pytest.raises(RuntimeError, match="must be"):
+                call(*(o.cpu().numpy() if j == i else o for j, o in enumerate(outs)))
+                pytest.fail(name)
