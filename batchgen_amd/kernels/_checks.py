@@ -84,11 +84,11 @@ def no_tangent(name: str, *tensors):
 def writable(name: str, *outs):
     """A caller's tensors that an op without a gradient is about to write: refused where autograd would go on with what
     they were (they require a gradient in grad mode, or carry a forward-mode tangent)."""
-    no_tangent(name, *outs)
-    if torch.is_grad_enabled():
-        for t in outs:
-            if t is not None and t.requires_grad:
-                fail(f"{name} writes its output without a gradient: the tensor it writes must not require one in grad mode")
+    if forward_ad._current_level >= 0:
+        no_tangent(name, *outs)
+    for t in outs:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            fail(f"{name} writes its output without a gradient: the tensor it writes must not require one in grad mode")
 
 
 def _span(t: torch.Tensor) -> int:
@@ -116,11 +116,9 @@ def apart(name: str, out: torch.Tensor, *operands, same_ok=()):
 
 def written(*outs):
     """Tells autograd that these tensors have been written, as torch's own in-place operations do: the backward pass of
-    an earlier graph that saved one of them then raises instead of using the new values.  (Inference tensors have no
-    version and cannot be saved.)"""
-    for t in outs:
-        if t is not None and not t.is_inference():
-            _increment_version(t)
+    an earlier graph that saved one of them then raises instead of using the new values.  (Inference tensors, which
+    have no version and cannot be saved, are passed over.)"""
+    _increment_version(outs)
 
 
 def launch(device: torch.device, fn, *args):

@@ -91,9 +91,9 @@ def _run_sort(x, plan, out):
     h = x.size(1)
     if out is None:
         out = torch.empty((plan.capacity, h), dtype=x.dtype, device=x.device)
-    size = x.element_size()
+    size, meta = x.element_size(), ptr(plan.meta)
     ck.launch(x.device, lib().bgmoe_token_sort_rows, ptr(x), x.stride(0) * size, h * size, plan.num_tokens,
-              plan.top_k, ptr(plan.topk_pos), ptr(plan.meta), ptr(plan.meta) + 4 * plan.num_experts, plan.num_experts, plan.capacity,
+              plan.top_k, ptr(plan.topk_pos), meta, meta + 4 * plan.num_experts, plan.num_experts, plan.capacity,
               int(zero_rest), ptr(out))
     return out
 

@@ -59,7 +59,7 @@ def int8_quant_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
         if held[1] is not None:
             ck.apart("int8_quant_rows", scale, x2, out)
         ck.launch(x.device, lib().bgmoe_int8_quant_rows, ptr(x2), code, x2.stride(0), rows, k, ptr(out), ptr(scale))
-        ck.written(*held)
+        ck.written(*(t for t in held if t is not None))
     return out, scale
 
 
